@@ -15,7 +15,7 @@ from . import _build
 _lock = threading.Lock()
 _lib = None
 
-FLK_F32, FLK_F64, FLK_F32_BF16X3 = 0, 1, 2
+FLK_F32, FLK_F64, FLK_F32_BF16X3, FLK_F16, FLK_BF16 = 0, 1, 2, 3, 4
 FLK_GAUSSIAN, FLK_LAPLACIAN, FLK_MATERN32, FLK_MATERN52, FLK_LAPLACIAN_DU = 0, 1, 2, 3, 4
 FLK_EINVAL, FLK_ENOMEM, FLK_EUNSUPPORTED, FLK_EHIP = -1, -2, -3, -4
 
@@ -71,6 +71,12 @@ _SIGNATURES["flk_tri_solve"] = (c_int, [c_int, c_int, c_void_p, c_int64, c_int64
                                         c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p])
 _SIGNATURES["flk_potrf_tile_rows"] = (c_int64, [c_int])
 _SIGNATURES["flk_potrf_tile"] = (c_int, [c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p])
+_SIGNATURES["flk_layer_norm"] = (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, ctypes.c_double,
+                                         c_void_p, c_void_p, c_void_p, c_int, c_void_p])
+_SIGNATURES["flk_layer_norm_backward_workspace_bytes"] = (c_size_t, [c_int64, c_int64, c_int])
+_SIGNATURES["flk_layer_norm_backward"] = (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int,
+                                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                                  c_void_p, c_size_t, c_void_p])
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
 

@@ -35,6 +35,9 @@ extern "C" {
 #define FLK_F32 0
 #define FLK_F64 1
 #define FLK_F32_BF16X3 2
+/* 16-bit data: the operators at the end of this file only */
+#define FLK_F16 3
+#define FLK_BF16 4
 
 /* Radial kernels K(x, c) = f(D), D = |x/sigma - c/sigma| (falkon/kernels/distance_kernel.py):
  * Gaussian exp(-D^2/2) (:140-159), Laplacian exp(-D) (:182-205), Matern nu = 3/2 and 5/2 (:225-269;
@@ -288,6 +291,25 @@ int flk_kernel_fmm(int kernel, const void *X1, int64_t n, int64_t x1_rs, int64_t
                    const void *sigma, int64_t n_sigma,
                    void *out, int64_t out_rs, int64_t out_cs, int dtype, int compute_f64,
                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- layer norm --------------------------------------------------------------
+ * flk_layer_norm: y = (x - mean) / sqrt(var + eps) * weight + bias, row by row (var: the mean of the squared distances
+ * from the mean).  x: rows x d at x[i*x_rs + k]; y: rows x d, contiguous, may not overlap x.  weight, bias: d values
+ * each or NULL, both of weight_dtype, which is dtype or, for 16-bit data, FLK_F32.  mean, rstd: one value a row for the
+ * backward pass (float; double for FLK_F64), or both NULL.  dtype: FLK_F32, FLK_F64, FLK_F16 or FLK_BF16; sums are held
+ * in float (double for FLK_F64) and rounded once.
+ * flk_layer_norm_backward: from dy (rows x d at dy[i*dy_rs + k]) and the forward pass's x, mean and rstd, the gradients dx
+ * (rows x d, contiguous), dweight and dbias (d values of weight_dtype); any of the three may be NULL.  The sums over the
+ * rows go through the workspace (none needed where both are NULL) in a fixed order: results are the same run to run. */
+int flk_layer_norm(const void *x, int64_t rows, int64_t d, int64_t x_rs, const void *weight, const void *bias,
+                   int weight_dtype, double eps, void *y, void *mean, void *rstd, int dtype, void *stream);
+
+size_t flk_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d, int dtype);
+
+int flk_layer_norm_backward(const void *x, int64_t rows, int64_t d, int64_t x_rs, const void *dy, int64_t dy_rs,
+                            const void *weight, int weight_dtype, const void *mean, const void *rstd,
+                            void *dx, void *dweight, void *dbias, int dtype,
+                            void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
