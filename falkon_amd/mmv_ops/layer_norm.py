@@ -104,8 +104,6 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TypeError(f"layer_norm takes float32, float64, float16 or bfloat16 tensors, not {getattr(x, 'dtype', type(x))}")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("layer_norm needs at least one feature")
-    if x.device.type != "cuda":
-        raise RuntimeError("layer_norm runs on the GPU only: tensors must be on a ROCm device")
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
@@ -120,6 +118,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             raise TypeError(f"{name} must be of the type of x or, for 16-bit x, float32, not {t.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must be of one type")
+    if x.device.type != "cuda":
+        raise RuntimeError("layer_norm runs on the GPU only: tensors must be on a ROCm device")
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
