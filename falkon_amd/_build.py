@@ -25,7 +25,9 @@ PER_KERNEL_FN = ["mmv_small_f32.hip", "mmv_small_f32_fold.hip", "mmv_small_f32_w
 SOURCES = [(src, kf) for src in PER_KERNEL_FN for kf in KERNEL_FNS]
 SOURCES.sort(key=lambda job: {"mmv_small_f32_wide.hip": 0, "mmv_small_f32.hip": 1, "mmv_small_f32_fold.hip": 2}.get(job[0], 3))
 SOURCES += [("api.hip", None), ("pack.hip", None), ("pack_split.hip", None), ("cg.hip", None), ("trsv.hip", None), ("potrf.hip", None),
-            ("layer_norm.hip", None)]
+            ("layer_norm.hip", None), ("attention.hip", None)]
+# The attention kernels are compiled once per element type: -DFLK_KF=0..2 (float32, float16, bfloat16).
+SOURCES += [(src, kf) for src in ("attention_bwd.hip", "attention_fwd.hip", "attention_cached.hip") for kf in (0, 1, 2)]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",

@@ -1,0 +1,253 @@
+// extern "C" entry points of the attention operators: argument checks, workspaces, launch plans, and the small kernels beside
+// them (document spans, sums of parts).
+#include "attention_common.h"
+
+namespace flk {
+
+// Smallest and largest document id of every kDocBlock positions; a padding position (a negative id) counts as -1.
+__global__ void __launch_bounds__(kAttnThreads) attention_doc_kernel(const int *docs, int64_t docs_b, int n, int blocks, int64_t total, int2 *out) {
+    const int64_t i = (int64_t)blockIdx.x * (kAttnThreads / kDocBlock) + threadIdx.x / kDocBlock;
+    const int64_t b = (i < total ? i : 0) / blocks;
+    const int pos = (int)((i < total ? i : 0) % blocks) * kDocBlock + threadIdx.x % kDocBlock;
+    const int id = pos < n ? max(docs[b * docs_b + pos], -1) : 0;
+    int lo = pos < n ? id : 0x7fffffff, hi = pos < n ? id : -1;
+#pragma unroll
+    for (int o = kDocBlock / 2; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
+    if (i < total && threadIdx.x % kDocBlock == 0) out[i] = {lo, hi};
+}
+
+// dslopes[h]: the workgroups' sums, in double and in a fixed order (their terms cancel)
+__global__ void __launch_bounds__(kAttnThreads) attention_dslopes_kernel(const float *part, int64_t n, float *out) {
+    __shared__ double lds[kAttnThreads];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kAttnThreads) s += (double)part[blockIdx.x * n + i];
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = kAttnThreads / 2; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) lds[threadIdx.x] += lds[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) out[blockIdx.x] = (float)lds[0];
+}
+
+// dk or dv from its parts
+template <typename T>
+__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(const float *part, int64_t n, int parts, T *out) {
+    for (int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kAttnThreads) {
+        float s = 0.f;
+        for (int k = 0; k < parts; k++) s += part[k * n + i];
+        out[i] = (T)s;
+    }
+}
+
+constexpr int64_t kMaxPositions = (int64_t)1 << 28;
+constexpr int64_t kMaxGrid = 0x7fffffff;
+static int elem_size(int dtype) { return dtype == FLK_F32 ? 4 : 2; }
+static bool attn_dtype(int dtype) { return dtype == FLK_F32 || dtype == FLK_F16 || dtype == FLK_BF16; }
+static int padded_d(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static bool rows_aligned(const void *p, const AttnStride &s, int64_t d, int es) {
+    const int64_t e = 16 / es;
+    return ((uintptr_t)p & 15) == 0 && s.b % e == 0 && s.s % e == 0 && s.h % e == 0 && d % e == 0;
+}
+
+struct AttnSizes { int64_t doc_blocks, docs, delta, slopes, parts; int splits; };
+static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, bool docs, bool slopes) {
+    AttnSizes z = {};
+    z.doc_blocks = cdiv(sk, kDocBlock);
+    z.docs = docs ? align256((size_t)(b * z.doc_blocks) * sizeof(int2)) : 0;
+    z.delta = align256((size_t)(b * hq * sq) * 4);
+    z.slopes = slopes ? align256((size_t)(b * hq * cdiv(sq, kAttnRows)) * 4) : 0;
+    // The dk / dv kernel has one workgroup for 128 keys of a key head; where that leaves compute units idle, the query heads
+    // that share the key head are divided over several, whose parts are added afterwards.
+    const int64_t groups = b * hk * cdiv(sk, kAttnRows), group = hk > 0 ? hq / hk : 1;
+    z.splits = 1;
+    if (groups > 0 && groups < 512) z.splits = (int)(cdiv(512, groups) < group ? cdiv(512, groups) : group);
+    if (z.splits < 1) z.splits = 1;
+    z.parts = z.splits > 1 ? align256((size_t)z.splits * b * sk * hk * (d + dv) * 4) : 0;
+    return z;
+}
+
+static int attn_check(const char *what, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, double softcap,
+                      int causal, const int *prefix, const int *docs, int dtype) {
+    if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1) return fail(FLK_EINVAL, "%s: bad shape", what);
+    if (hq % hk != 0) return fail(FLK_EINVAL, "%s: %lld query heads cannot share %lld key heads evenly", what, (long long)hq, (long long)hk);
+    if (!attn_dtype(dtype)) return fail(FLK_EINVAL, "%s: unknown dtype %d", what, dtype);
+    if (d > kAttnMaxD || dv > kAttnMaxD) return fail(FLK_EUNSUPPORTED, "%s: heads of more than %d values", what, kAttnMaxD);
+    if (sq > kMaxPositions || sk > kMaxPositions) return fail(FLK_EUNSUPPORTED, "%s: more than %lld positions", what, (long long)kMaxPositions);
+    if (!(softcap >= 0.0)) return fail(FLK_EINVAL, "%s: softcap must not be negative", what);
+    if (prefix != nullptr && !causal) return fail(FLK_EINVAL, "%s: a prefix belongs to a causal mask", what);
+    if (docs != nullptr && sq > sk) return fail(FLK_EINVAL, "%s: documents need every query to stand at a key's position", what);
+    if (b > 0 && (hq > kMaxGrid / b || b * hq * cdiv(sq > sk ? sq : sk, kAttnRows) > kMaxGrid))
+        return fail(FLK_EUNSUPPORTED, "%s: too many rows for one launch", what);
+    return FLK_OK;
+}
+
+static int launch_docs(const AttnArgs &a, hipStream_t st) {
+    const int64_t total = (int64_t)a.b * a.doc_blocks;
+    if (a.docs == nullptr || total == 0) return FLK_OK;
+    hipLaunchKernelGGL(attention_doc_kernel, dim3((unsigned)cdiv(total, kAttnThreads / kDocBlock)), dim3(kAttnThreads), 0, st, a.docs,
+                       a.docs_b, a.sk, a.doc_blocks, total, a.doc_range);
+    FLK_LAUNCH_CHECK("attention_doc_kernel");
+    return FLK_OK;
+}
+
+template <typename T> static int attention_backward_impl(AttnArgs &a, int dp, float *dslopes, hipStream_t st) {
+    int rc = FLK_OK;
+    if ((int64_t)a.b * a.sq > 0 && (rc = launch_attention_dq<T>(a, dp, st)) != FLK_OK) return rc;
+    if (dslopes != nullptr) {
+        hipLaunchKernelGGL(attention_dslopes_kernel, dim3((unsigned)a.hq), dim3(kAttnThreads), 0, st, a.dslopes_part,
+                           (int64_t)a.b * cdiv(a.sq, kAttnRows), dslopes);
+        FLK_LAUNCH_CHECK("attention_dslopes_kernel");
+    }
+    if (a.dk == nullptr || (int64_t)a.b * a.sk == 0) return FLK_OK;
+    if ((rc = launch_attention_dkv<T>(a, dp, st)) != FLK_OK || a.splits == 1) return rc;
+    const int64_t nk = (int64_t)a.b * a.sk * a.hk * a.d, nv = (int64_t)a.b * a.sk * a.hk * a.dv_d;
+    const auto grid = [](int64_t n) { return dim3((unsigned)(cdiv(n, kAttnThreads) < 4096 ? cdiv(n, kAttnThreads) : 4096)); };
+    hipLaunchKernelGGL((attention_join_kernel<T>), grid(nk), dim3(kAttnThreads), 0, st, a.dkv_part, nk, a.splits, (T *)a.dk);
+    hipLaunchKernelGGL((attention_join_kernel<T>), grid(nv), dim3(kAttnThreads), 0, st, a.dkv_part + a.splits * nk, nv, a.splits, (T *)a.dv);
+    FLK_LAUNCH_CHECK("attention_join_kernel");
+    return FLK_OK;
+}
+
+// Workgroups the keys of a sequence are divided over: enough to fill the chip from the shortest calls on, and no more than
+// one per four tiles of a wave at the cache's capacity.
+static int cached_splits(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk) {
+    const int64_t groups = b * hk * cdiv(t * (hq / hk), 32);
+    const int64_t most = cdiv(capacity, 4 * 4 * kCachedKeys);
+    int64_t n = groups > 0 ? cdiv(2048, groups) : 1;
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+
+}  // namespace flk
+
+using namespace flk;
+
+#define FLK_BY_TYPE(dtype, CALL)                       \
+    (dtype == FLK_F32 ? CALL(float) : dtype == FLK_F16 ? CALL(f16_t) : CALL(bf16_t))
+
+extern "C" {
+
+int64_t flk_attention_max_d(int dtype) { return attn_dtype(dtype) ? kAttnMaxD : 0; }
+
+size_t flk_attention_workspace_bytes(int64_t b, int64_t sk, int with_documents) {
+    if (b < 0 || sk < 0 || sk > kMaxPositions || !with_documents) return 0;
+    return align256((size_t)(b * cdiv(sk, kDocBlock)) * sizeof(int2));
+}
+
+int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                  const void *v, int64_t v_b, int64_t v_s, int64_t v_h, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk,
+                  int64_t d, int64_t dv, double scale, double softcap, const float *slopes, int causal, const int *prefix,
+                  const int *documents, int64_t documents_b, void *out, float *lse, int dtype, void *workspace,
+                  size_t workspace_bytes, void *stream) {
+    fail(FLK_OK, "%s", "");
+    int rc = attn_check("flk_attention", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
+    if (rc != FLK_OK || b * sq == 0) return rc;
+    if (q == nullptr || out == nullptr || (sk > 0 && (k == nullptr || v == nullptr))) return fail(FLK_EINVAL, "flk_attention: null pointer");
+    const size_t need = flk_attention_workspace_bytes(b, sk, documents != nullptr);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+    AttnArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse;
+    a.qs = {q_b, q_s, q_h}; a.ks = {k_b, k_s, k_h}; a.vs = {v_b, v_s, v_h};
+    a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
+    a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
+    a.docs = documents; a.docs_b = documents_b; a.doc_range = (int2 *)workspace; a.doc_blocks = (int)cdiv(sk, kDocBlock);
+    const int es = elem_size(dtype);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es);
+    hipStream_t st = (hipStream_t)stream;
+    if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
+    const int dp = padded_d(d > dv ? d : dv);
+#define FLK_CALL(T) launch_attention_fwd<T>(a, dp, st)
+    return FLK_BY_TYPE(dtype, FLK_CALL);
+#undef FLK_CALL
+}
+
+size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                                              int with_slopes, int with_documents) {
+    if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1 || hq % hk != 0 || sq > kMaxPositions || sk > kMaxPositions) return 0;
+    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, with_documents != 0, with_slopes != 0);
+    return (size_t)(z.docs + z.delta + z.slopes + z.parts);
+}
+
+int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const float *lse, const void *dout,
+                           int64_t do_b, int64_t do_s, int64_t do_h, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d,
+                           int64_t dv, double scale, double softcap, const float *slopes, int causal, const int *prefix,
+                           const int *documents, int64_t documents_b, void *dq, void *dk, void *dv_out, float *dslopes, int dtype,
+                           void *workspace, size_t workspace_bytes, void *stream) {
+    fail(FLK_OK, "%s", "");
+    int rc = attn_check("flk_attention_backward", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
+    if (rc != FLK_OK) return rc;
+    if ((dk == nullptr) != (dv_out == nullptr)) return fail(FLK_EINVAL, "flk_attention_backward: dk and dv come together");
+    if (dslopes != nullptr && slopes == nullptr) return fail(FLK_EINVAL, "flk_attention_backward: no slopes to differentiate");
+    if ((b * sq > 0 && (q == nullptr || out == nullptr || lse == nullptr || dout == nullptr)) || (b * sk > 0 && (k == nullptr || v == nullptr)))
+        return fail(FLK_EINVAL, "flk_attention_backward: null pointer");
+    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, documents != nullptr, dslopes != nullptr);
+    const size_t need = (size_t)(z.docs + z.delta + z.slopes + z.parts);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+    AttnArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = (float *)lse; a.dq = dq; a.dk = dk; a.dv = dv_out;
+    a.qs = {q_b, q_s, q_h}; a.ks = {k_b, k_s, k_h}; a.vs = {v_b, v_s, v_h};
+    a.os = {sq * hq * dv, hq * dv, dv}; a.dos = {do_b, do_s, do_h};
+    a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
+    a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
+    a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)z.doc_blocks; a.splits = z.splits;
+    char *ws = (char *)workspace;
+    a.doc_range = (int2 *)ws; ws += z.docs;
+    a.delta = (float *)ws; ws += z.delta;
+    a.dslopes_part = dslopes != nullptr ? (float *)ws : nullptr; ws += z.slopes;
+    a.dkv_part = (float *)ws;
+    const int es = elem_size(dtype);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) &&
+            rows_aligned(out, a.os, dv, es) && rows_aligned(dout, a.dos, dv, es);
+    hipStream_t st = (hipStream_t)stream;
+    if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
+    const int dp = padded_d(d > dv ? d : dv);
+#define FLK_CALL(T) attention_backward_impl<T>(a, dp, dslopes, st)
+    return FLK_BY_TYPE(dtype, FLK_CALL);
+#undef FLK_CALL
+}
+
+size_t flk_attention_cached_workspace_bytes(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk, int64_t dv) {
+    if (b < 0 || t < 0 || capacity < 0 || hq < 1 || hk < 1 || dv < 1 || hq % hk != 0) return 0;
+    const int64_t n = cached_splits(b, t, capacity, hq, hk);
+    return n > 1 ? align256((size_t)(b * t * hq * n * dv) * 4) + align256((size_t)(b * t * hq * n * 2) * 4) : 0;
+}
+
+int flk_attention_cached(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                         const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const int *lengths, int64_t b, int64_t t,
+                         int64_t capacity, int64_t hq, int64_t hk, int64_t d, int64_t dv, double scale, double softcap,
+                         const float *slopes, void *out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    fail(FLK_OK, "%s", "");
+    int rc = attn_check("flk_attention_cached", b, t, capacity, hq, hk, d, dv, softcap, 1, nullptr, nullptr, dtype);
+    if (rc != FLK_OK || b * t == 0) return rc;
+    if (q == nullptr || out == nullptr || lengths == nullptr || (capacity > 0 && (k == nullptr || v == nullptr)))
+        return fail(FLK_EINVAL, "flk_attention_cached: null pointer");
+    const int64_t n = cached_splits(b, t, capacity, hq, hk);
+    const size_t need = flk_attention_cached_workspace_bytes(b, t, capacity, hq, hk, dv);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+    CachedArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.out = out;
+    a.qs = {q_b, q_s, q_h}; a.ks = {k_b, k_s, k_h}; a.vs = {v_b, v_s, v_h};
+    a.lengths = lengths; a.slopes = slopes;
+    a.part_o = (float *)workspace;
+    a.part_ml = (float *)((char *)workspace + (n > 1 ? align256((size_t)(b * t * hq * n * dv) * 4) : 0));
+    a.b = (int)b; a.t = (int)t; a.capacity = (int)capacity; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d;
+    a.dv_d = (int)dv; a.splits = (int)n; a.blocks_r = (int)cdiv(t * (hq / hk), 32); a.scale = (float)scale; a.cap = (float)softcap;
+    const int64_t grid = b * hk * a.blocks_r * n;
+    if (grid > kMaxGrid || cdiv(b * t * hq * dv, kAttnThreads) > kMaxGrid) return fail(FLK_EUNSUPPORTED, "flk_attention_cached: too many rows for one launch");
+    const int es = elem_size(dtype);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es);
+    hipStream_t st = (hipStream_t)stream;
+    const int dp = padded_d(d > dv ? d : dv);
+#define FLK_CALL(T) launch_attention_cached<T>(a, dp, st)
+    return FLK_BY_TYPE(dtype, FLK_CALL);
+#undef FLK_CALL
+}
+
+}  // extern "C"

@@ -1,0 +1,193 @@
+// Attention of the newest tokens of ragged sequences over a cache of keys and values (gfx950).  Compiled once per element type.
+//
+// Bound by reading the cache once.  The query rows that read the same keys (the heads that share a key head, times the new
+// tokens) are packed into the 32 columns of the matrix instructions, so that products cost little beside the reads, and the
+// keys of a sequence are divided over workgroups and over a workgroup's four waves.  Every wave walks over tiles of 32 keys of
+// its own with no barrier: the next tile's reads are in flight, in registers, while the present one is used from LDS.  The waves'
+// results meet in LDS, those of several workgroups in a second kernel, both in a fixed order.
+#include "attention_common.h"
+
+namespace flk {
+
+template <typename T, int DP, bool MOD>
+__global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_cached_kernel(CachedArgs p) {
+    typedef AttnType<T> AT;
+    typedef typename AT::frag frag;
+    typedef Tile<T, DP> TL;
+    constexpr int TK = kCachedKeys, C = DP / AT::KS, DB = DP / 32, ST = 32 / AT::KS, NC = TL::NC, N = TK * NC / 64;
+    constexpr int kWave = 2 * TK * TL::RB, kJoin = 32 * (DP + 1) * 4;          // LDS of a wave: its tiles, later its output
+    constexpr int kLds = kWave > kJoin ? kWave : kJoin;
+    __shared__ __align__(16) char lds[4 * kLds];
+    __shared__ float lds_ml[4][32][2];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int pairs = p.b * p.hk;
+    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs, rb = rest % p.blocks_r, split = rest / p.blocks_r;
+    const int b = pair / p.hk, hk = pair % p.hk;
+    const int len = max(0, min(p.lengths[b], p.capacity));
+    const int n_rows = p.t * p.group;
+    const int r = rb * 32 + (lane & 31);
+    const bool live = r < n_rows;
+    const int t = r / p.group, h = hk * p.group + r % p.group;
+    const int pos = len - p.t + t, pos_lo = len - p.t + rb * 32 / p.group;
+    const float slope = MOD && p.slopes != nullptr && live ? p.slopes[h] : 0.f;
+    // this workgroup's keys, in whole tiles
+    const int all = (len + TK - 1) / TK, per = (all + p.splits - 1) / p.splits;
+    const int tile_lo = min(split * per, all), tile_hi = min(tile_lo + per, all);
+
+    const T *qrow = (const T *)p.q + b * p.qs.b + (int64_t)t * p.qs.s + h * p.qs.h;
+    const T *kbase = (const T *)p.k + b * p.ks.b + hk * p.ks.h;
+    const T *vbase = (const T *)p.v + b * p.vs.b + hk * p.vs.h;
+    char *lds_k = lds + wave * kLds, *lds_v = lds_k + TK * TL::RB;
+    frag qf[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        union { ux4 u; frag f; } x;
+        x.u = load_chunk<T>(qrow, 2 * c + half, p.d, live, p.vec);
+        qf[c] = x.f;
+    }
+    fx16 o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++) o[db] = fx16{};
+    float m = -kInf, l = 0.f;
+
+    ux4 rk[N], rv[N];
+    auto fetch = [&](int tile) {
+        const int k0 = tile * TK;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int i = n * 64 + lane, row = k0 + i / NC, c = i % NC;
+            rk[n] = load_chunk<T>(kbase + row * p.ks.s, c, p.d, row < len, p.vec);
+            rv[n] = load_chunk<T>(vbase + row * p.vs.s, c, p.dv_d, row < len, p.vec);
+        }
+    };
+    int tile = tile_lo + wave;
+    if (tile < tile_hi) fetch(tile);
+    for (; tile < tile_hi; tile += 4) {
+        const int k0 = tile * TK;
+        const bool full = k0 + TK - 1 <= pos_lo;
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int i = n * 64 + lane, row = i / NC, c = i % NC;
+            *(ux4 *)(lds_k + TL::at(row, c)) = rk[n];
+            *(ux4 *)(lds_v + TL::at(row, c)) = rv[n];
+            if (!full) bad |= any_nonfinite<T>(rv[n]);
+        }
+        const bool careful = !full && __any(bad);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (tile + 4 < tile_hi) fetch(tile + 4);
+        fx16 s = {};
+#pragma unroll
+        for (int c = 0; c < C; c++) s = AT::mma(TL::rows(lds_k, 0, c), qf[c], s);
+        float top = -kInf;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int key = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
+            float th, x;
+            if constexpr (!MOD) x = s[i] * (p.scale * kScoreUnit);
+            else {
+                x = s[i] * p.scale;
+                if (p.cap > 0.f) { th = tanh_of<T>(x * __builtin_amdgcn_rcpf(p.cap)); x = p.cap * th; }
+                x = (x - slope * __builtin_fabsf((float)(pos - key))) * kScoreUnit;
+            }
+            if (!full) x = key <= pos ? x : -kInf;                 // pos < len: nothing behind the sequence either
+            s[i] = x;
+            top = fmaxf(top, x);
+        }
+        top = fmaxf(top, other_half(top));
+        if (__any(top > m)) {
+            const float next = fmaxf(m, top);
+            const float a = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - next);
+            l *= a;
+            m = next;
+#pragma unroll
+            for (int db = 0; db < DB; db++) o[db] *= a;
+        }
+        const float base_m = m == -kInf ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < 16; i++) { s[i] = __builtin_amdgcn_exp2f(s[i] - base_m); l += s[i]; }
+#pragma unroll
+        for (int st = 0; st < ST; st++) {
+            const frag pf = pack<T>(s, st);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const frag vf = TL::cols(lds_v, AT::KS * st, 32 * db);
+                if (careful) o[db] = mma_careful<T>(vf, pf, o[db]);
+                else o[db] = AT::mma(vf, pf, o[db]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    l += other_half(l);
+
+    // the four waves' results: o relative to the largest of their maxima
+    float *mine = (float *)(lds + wave * kLds);
+    __syncthreads();
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mine[(lane & 31) * (DP + 1) + 32 * db + 8 * (i >> 2) + 4 * half + (i & 3)] = o[db][i];
+    if (half == 0) { lds_ml[wave][lane][0] = m; lds_ml[wave][lane][1] = l; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * DP; i += kAttnThreads) {
+        const int rr = i / DP, c = i % DP, row = rb * 32 + rr;
+        if (row >= n_rows || c >= p.dv_d) continue;
+        const float top = fmaxf(fmaxf(lds_ml[0][rr][0], lds_ml[1][rr][0]), fmaxf(lds_ml[2][rr][0], lds_ml[3][rr][0]));
+        float x = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float mw = lds_ml[w][rr][0];
+            if (mw == -kInf && lds_ml[w][rr][1] == 0.f) continue;  // saw nothing
+            const float a = mw == -kInf ? 1.f : __builtin_amdgcn_exp2f(mw - top);
+            x += a * ((const float *)(lds + w * kLds))[rr * (DP + 1) + c];
+            sum += a * lds_ml[w][rr][1];
+        }
+        const int tt = row / p.group, hh = hk * p.group + row % p.group;
+        const int64_t at = ((int64_t)b * p.t + tt) * p.hq + hh;
+        if (p.splits == 1) ((T *)p.out)[at * p.dv_d + c] = (T)(sum == 0.f ? 0.f : x / sum);
+        else {
+            p.part_o[(at * p.splits + split) * p.dv_d + c] = x;
+            if (c == 0) { p.part_ml[(at * p.splits + split) * 2] = top; p.part_ml[(at * p.splits + split) * 2 + 1] = sum; }
+        }
+    }
+}
+
+// out from the parts of `splits` workgroups, one thread a value
+template <typename T>
+__global__ void __launch_bounds__(kAttnThreads) attention_cached_join_kernel(CachedArgs p) {
+    const int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x;
+    if (i >= (int64_t)p.b * p.t * p.hq * p.dv_d) return;
+    const int64_t row = i / p.dv_d, c = i % p.dv_d;
+    const float *ml = p.part_ml + row * p.splits * 2, *po = p.part_o + row * p.splits * p.dv_d + c;
+    float top = -kInf;
+    for (int s = 0; s < p.splits; s++) top = fmaxf(top, ml[2 * s]);
+    float x = 0.f, sum = 0.f;
+    for (int s = 0; s < p.splits; s++) {
+        if (ml[2 * s] == -kInf && ml[2 * s + 1] == 0.f) continue;
+        const float a = ml[2 * s] == -kInf ? 1.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
+        x += a * po[(int64_t)s * p.dv_d];
+        sum += a * ml[2 * s + 1];
+    }
+    ((T *)p.out)[i] = (T)(sum == 0.f ? 0.f : x / sum);
+}
+
+#define FLK_CACHED(DP)                                                                                                           \
+    if (a.cap > 0.f || a.slopes != nullptr) hipLaunchKernelGGL((attention_cached_kernel<T, DP, true>), grid, dim3(kAttnThreads), 0, st, a); \
+    else hipLaunchKernelGGL((attention_cached_kernel<T, DP, false>), grid, dim3(kAttnThreads), 0, st, a);
+template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.blocks_r * a.splits));
+    if (dp == 32) { FLK_CACHED(32) } else if (dp == 64) { FLK_CACHED(64) } else if (dp == 96) { FLK_CACHED(96) } else { FLK_CACHED(128) }
+    FLK_LAUNCH_CHECK("attention_cached_kernel");
+    if (a.splits > 1) {
+        const int64_t n = (int64_t)a.b * a.t * a.hq * a.dv_d;
+        hipLaunchKernelGGL((attention_cached_join_kernel<T>), dim3((unsigned)((n + kAttnThreads - 1) / kAttnThreads)), dim3(kAttnThreads), 0, st, a);
+        FLK_LAUNCH_CHECK("attention_cached_join_kernel");
+    }
+    return FLK_OK;
+}
+template int launch_attention_cached<attn_t>(const CachedArgs &, int, hipStream_t);
+
+}  // namespace flk

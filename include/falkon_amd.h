@@ -311,6 +311,52 @@ int flk_layer_norm_backward(const void *x, int64_t rows, int64_t d, int64_t x_rs
                             void *dx, void *dweight, void *dbias, int dtype,
                             void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- attention -----------------------------------------------------------------
+ * out_i = sum_j softmax_j(x_ij) v_j over the keys j that row i sees, matrix-free, where
+ *   x = scale * q_i.k_j;  x <- softcap * tanh(x / softcap) if softcap > 0;  x <- x - slopes[h] * |pos_i - j| if slopes
+ * and pos_i = i + sk - sq (the queries are the newest positions).  A row that sees nothing is zero.
+ * q, k, v: b x rows x heads x values with strides (in elements) of batch, row and head; the values of a row are next to
+ * each other.  hq is a multiple of hk; heads up to flk_attention_max_d values.  dtype: FLK_F32, FLK_F16 or FLK_BF16.
+ * causal: keys behind pos_i are hidden, except the first prefix[b] of them (prefix: b ints or NULL, causal only).
+ * documents: b x sk ints (rows documents_b apart) or NULL: a row sees keys of its own number only, and nothing if that
+ * is negative; needs sq <= sk.  out: b x sq x hq x dv, contiguous.  lse: b x hq x sq floats (the logarithm of the row's sum,
+ * -inf for a row that sees nothing), or NULL where no backward pass follows.
+ * flk_attention_backward: from out, lse and dout the gradients dq, dk, dv (contiguous, like q, k, v; dk and dv both or
+ * neither) and dslopes (hq floats); each may be NULL.  Sums are made in a fixed order: the same run to run. */
+int64_t flk_attention_max_d(int dtype);
+
+size_t flk_attention_workspace_bytes(int64_t b, int64_t sk, int with_documents);
+
+int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                  const void *v, int64_t v_b, int64_t v_s, int64_t v_h,
+                  int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                  double scale, double softcap, const float *slopes, int causal, const int *prefix,
+                  const int *documents, int64_t documents_b, void *out, float *lse, int dtype,
+                  void *workspace, size_t workspace_bytes, void *stream);
+
+size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                                              int with_dslopes, int with_documents);
+
+int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const float *lse,
+                           const void *dout, int64_t do_b, int64_t do_s, int64_t do_h,
+                           int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                           double scale, double softcap, const float *slopes, int causal, const int *prefix,
+                           const int *documents, int64_t documents_b, void *dq, void *dk, void *dv_out, float *dslopes,
+                           int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same for the newest t tokens of sequences of different lengths over a cache: k, v are b x capacity x heads x values,
+ * lengths (b ints in device memory) the keys each sequence has, new tokens included; token i of t stands at
+ * lengths[b] - t + i and sees the keys up to there.  Lengths outside [0, capacity] count as the nearest of the two;
+ * keys behind a sequence's end are not read.  out: b x t x hq x dv, contiguous. */
+size_t flk_attention_cached_workspace_bytes(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk, int64_t dv);
+
+int flk_attention_cached(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
+                         const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const int *lengths,
+                         int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                         double scale, double softcap, const float *slopes, void *out, int dtype,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
