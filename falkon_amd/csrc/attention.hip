@@ -4,16 +4,20 @@
 
 namespace flk {
 
-// Smallest and largest document id of every kDocBlock positions; a padding position (a negative id) counts as -1.
-__global__ void __launch_bounds__(kAttnThreads) attention_doc_kernel(const int *docs, int64_t docs_b, int n, int blocks, int64_t total, int2 *out) {
+// Smallest and largest document id of every kDocBlock positions, a padding position (a negative id) counting as -1; and the ids
+// themselves, row after row from a multiple of 16 bytes on, -1 for padding and past the end.
+__global__ void __launch_bounds__(kAttnThreads) attention_doc_kernel(const int *docs, int64_t docs_b, int n, int blocks, int64_t total, int2 *out,
+                                                                     int *ids) {
     const int64_t i = (int64_t)blockIdx.x * (kAttnThreads / kDocBlock) + threadIdx.x / kDocBlock;
     const int64_t b = (i < total ? i : 0) / blocks;
     const int pos = (int)((i < total ? i : 0) % blocks) * kDocBlock + threadIdx.x % kDocBlock;
-    const int id = pos < n ? max(docs[b * docs_b + pos], -1) : 0;
-    int lo = pos < n ? id : 0x7fffffff, hi = pos < n ? id : -1;
+    const int id = pos < n ? max(docs[b * docs_b + pos], -1) : -1;
+    int lo = pos < n ? id : 0x7fffffff, hi = id;
 #pragma unroll
     for (int o = kDocBlock / 2; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
-    if (i < total && threadIdx.x % kDocBlock == 0) out[i] = {lo, hi};
+    if (i >= total) return;
+    ids[i * kDocBlock + threadIdx.x % kDocBlock] = id;
+    if (threadIdx.x % kDocBlock == 0) out[i] = {lo, hi};
 }
 
 // dslopes[h]: the workgroups' sums, in double and in a fixed order (their terms cancel)
@@ -49,15 +53,27 @@ static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static bool rows_aligned(const void *p, const AttnStride &s, int64_t d, int es) {
     const int64_t e = 16 / es;
+    if (s.s > ((int64_t)1 << 23) || s.s < 0) return false;        // a tile's offsets are 32 bits wide
     return ((uintptr_t)p & 15) == 0 && s.b % e == 0 && s.s % e == 0 && s.h % e == 0 && d % e == 0;
 }
 
-struct AttnSizes { int64_t doc_blocks, docs, delta, slopes, parts; int splits; };
+// document spans, then ids
+static int64_t doc_bytes(int64_t b, int64_t sk) {
+    const int64_t n = b * cdiv(sk, kDocBlock);
+    return align256((size_t)n * sizeof(int2)) + align256((size_t)n * kDocBlock * 4);
+}
+static void place_docs(AttnArgs &a, void *ws) {
+    a.doc_range = (int2 *)ws;
+    a.doc_ids = (int *)((char *)ws + align256((size_t)a.b * a.doc_blocks * sizeof(int2)));
+}
+
+struct AttnSizes { int64_t doc_blocks, docs, sq_pad, stats, slopes, parts; int splits; };
 static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, bool docs, bool slopes) {
     AttnSizes z = {};
     z.doc_blocks = cdiv(sk, kDocBlock);
-    z.docs = docs ? align256((size_t)(b * z.doc_blocks) * sizeof(int2)) : 0;
-    z.delta = align256((size_t)(b * hq * sq) * 4);
+    z.docs = docs ? doc_bytes(b, sk) : 0;
+    z.sq_pad = cdiv(sq, kAttnRows) * kAttnRows;
+    z.stats = align256((size_t)(b * hq * z.sq_pad) * 8);
     z.slopes = slopes ? align256((size_t)(b * hq * cdiv(sq, kAttnRows)) * 4) : 0;
     // The dk / dv kernel has one workgroup for 128 keys of a key head; where that leaves compute units idle, the query heads
     // that share the key head are divided over several, whose parts are added afterwards.
@@ -88,7 +104,7 @@ static int launch_docs(const AttnArgs &a, hipStream_t st) {
     const int64_t total = (int64_t)a.b * a.doc_blocks;
     if (a.docs == nullptr || total == 0) return FLK_OK;
     hipLaunchKernelGGL(attention_doc_kernel, dim3((unsigned)cdiv(total, kAttnThreads / kDocBlock)), dim3(kAttnThreads), 0, st, a.docs,
-                       a.docs_b, a.sk, a.doc_blocks, total, a.doc_range);
+                       a.docs_b, a.sk, a.doc_blocks, total, a.doc_range, a.doc_ids);
     FLK_LAUNCH_CHECK("attention_doc_kernel");
     return FLK_OK;
 }
@@ -134,13 +150,13 @@ int64_t flk_attention_max_d(int dtype) { return attn_dtype(dtype) ? kAttnMaxD : 
 
 size_t flk_attention_workspace_bytes(int64_t b, int64_t sk, int with_documents) {
     if (b < 0 || sk < 0 || sk > kMaxPositions || !with_documents) return 0;
-    return align256((size_t)(b * cdiv(sk, kDocBlock)) * sizeof(int2));
+    return (size_t)doc_bytes(b, sk);
 }
 
 int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
                   const void *v, int64_t v_b, int64_t v_s, int64_t v_h, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk,
                   int64_t d, int64_t dv, double scale, double softcap, const float *slopes, int causal, const int *prefix,
-                  const int *documents, int64_t documents_b, void *out, float *lse, int dtype, void *workspace,
+                  const int *documents, int64_t documents_b, void *out, void *rest, float *lse, int dtype, void *workspace,
                   size_t workspace_bytes, void *stream) {
     fail(FLK_OK, "%s", "");
     int rc = attn_check("flk_attention", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
@@ -150,11 +166,12 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     AttnArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse;
+    a.q = q; a.k = k; a.v = v; a.o = out; a.rest = dtype == FLK_F32 ? nullptr : rest; a.lse = lse;
     a.qs = {q_b, q_s, q_h}; a.ks = {k_b, k_s, k_h}; a.vs = {v_b, v_s, v_h};
     a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
     a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
-    a.docs = documents; a.docs_b = documents_b; a.doc_range = (int2 *)workspace; a.doc_blocks = (int)cdiv(sk, kDocBlock);
+    a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)cdiv(sk, kDocBlock);
+    place_docs(a, workspace);
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es);
     hipStream_t st = (hipStream_t)stream;
@@ -169,11 +186,11 @@ size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk,
                                               int with_slopes, int with_documents) {
     if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1 || hq % hk != 0 || sq > kMaxPositions || sk > kMaxPositions) return 0;
     const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, with_documents != 0, with_slopes != 0);
-    return (size_t)(z.docs + z.delta + z.slopes + z.parts);
+    return (size_t)(z.docs + z.stats + z.slopes + z.parts);
 }
 
 int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
-                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const float *lse, const void *dout,
+                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const void *rest, const float *lse, const void *dout,
                            int64_t do_b, int64_t do_s, int64_t do_h, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d,
                            int64_t dv, double scale, double softcap, const float *slopes, int causal, const int *prefix,
                            const int *documents, int64_t documents_b, void *dq, void *dk, void *dv_out, float *dslopes, int dtype,
@@ -186,24 +203,24 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     if ((b * sq > 0 && (q == nullptr || out == nullptr || lse == nullptr || dout == nullptr)) || (b * sk > 0 && (k == nullptr || v == nullptr)))
         return fail(FLK_EINVAL, "flk_attention_backward: null pointer");
     const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, documents != nullptr, dslopes != nullptr);
-    const size_t need = (size_t)(z.docs + z.delta + z.slopes + z.parts);
+    const size_t need = (size_t)(z.docs + z.stats + z.slopes + z.parts);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     AttnArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = (float *)lse; a.dq = dq; a.dk = dk; a.dv = dv_out;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.rest = dtype == FLK_F32 ? nullptr : (void *)rest; a.dout = dout; a.lse = (float *)lse; a.dq = dq; a.dk = dk; a.dv = dv_out;
     a.qs = {q_b, q_s, q_h}; a.ks = {k_b, k_s, k_h}; a.vs = {v_b, v_s, v_h};
-    a.os = {sq * hq * dv, hq * dv, dv}; a.dos = {do_b, do_s, do_h};
+    a.dos = {do_b, do_s, do_h}; a.sq_pad = z.sq_pad;
     a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
     a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
     a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)z.doc_blocks; a.splits = z.splits;
     char *ws = (char *)workspace;
-    a.doc_range = (int2 *)ws; ws += z.docs;
-    a.delta = (float *)ws; ws += z.delta;
+    place_docs(a, ws); ws += z.docs;
+    a.stats = (float *)ws; ws += z.stats;
     a.dslopes_part = dslopes != nullptr ? (float *)ws : nullptr; ws += z.slopes;
     a.dkv_part = (float *)ws;
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) &&
-            rows_aligned(out, a.os, dv, es) && rows_aligned(dout, a.dos, dv, es);
+            rows_aligned(out, a.vs, dv, es) && rows_aligned(a.rest, a.vs, dv, es) && rows_aligned(dout, a.dos, dv, es);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);

@@ -6,23 +6,23 @@
 //   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i P_ij dout_i
 //
 // Two kernels instead of one with atomic sums of dq: seven products instead of five, and gradients that are the same run to
-// run.  The first owns queries (dq, delta, the slopes' partial sums), the second keys (dk, dv; it walks over the query heads
-// that share its key head, so those are summed in registers).
+// run.  The first owns queries (dq, the rows' statistics, the slopes' partial sums), the second keys (dk, dv; it walks over
+// the query heads that share its key head, so those are summed in registers).
 #include "attention_common.h"
 
 namespace flk {
 
 template <typename T, int DP, bool MOD>
-__global__ void __launch_bounds__(kAttnThreads, 2) attention_dq_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
     constexpr int TK = AT::kTile, KB = TK / 32, C = DP / AT::KS, DB = DP / 32, ST = 32 / AT::KS;
-    __shared__ __align__(16) char lds_k[TK * TL::RB];
-    __shared__ __align__(16) char lds_v[TK * TL::RB];
+    typedef Feed<T, DP, TK> FD;
+    constexpr int kTileBytes = TK * TL::RB;
+    __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ int lds_doc[8];
     __shared__ float lds_sum[4];
-    __shared__ int lds_bad;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int heads = p.b * p.hq, pairs = p.b * p.hk;
@@ -32,112 +32,150 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_dq_kernel(AttnArgs 
     const int off = p.sk - p.sq;
     const int i0 = tile_q * kAttnRows, row = i0 + wave * 32 + (lane & 31);
     const bool live = row < p.sq;
-    const int pos = row + off;
-    const int pos_lo = i0 + wave * 32 + off;
+    const int pos = row + off, pos_lo = i0 + wave * 32 + off;
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;
     const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
     const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;
 
+    typename TL::Lane at_lane;
+    at_lane.init();
+    FD feed_k, feed_v;
+    feed_k.init((const T *)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, p.d, p.vec);
+    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec);
     const T *qrow = (const T *)p.q + b * p.qs.b + h * p.qs.h + (int64_t)row * p.qs.s;
-    const T *orow = (const T *)p.out + b * p.os.b + h * p.os.h + (int64_t)row * p.os.s;
     const T *grow = (const T *)p.dout + b * p.dos.b + h * p.dos.h + (int64_t)row * p.dos.s;
-    const T *kbase = (const T *)p.k + b * p.ks.b + hk * p.ks.h;
-    const T *vbase = (const T *)p.v + b * p.vs.b + hk * p.vs.h;
+    const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
     frag qf[C], gf[C];
     float delta = 0.f;
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        union { ux4 u; frag f; } x, g, o;
+        union { ux4 u; frag f; } x, g, o, e;
         x.u = load_chunk<T>(qrow, 2 * c + half, p.d, live, p.vec);
         g.u = load_chunk<T>(grow, 2 * c + half, p.dv_d, live, p.vec);
-        o.u = load_chunk<T>(orow, 2 * c + half, p.dv_d, live, p.vec);
+        o.u = load_chunk<T>((const T *)p.out + at, 2 * c + half, p.dv_d, live, p.vec);
+        e.u = load_chunk<T>((const T *)p.rest + at, 2 * c + half, p.dv_d, live && p.rest != nullptr, p.vec);
         qf[c] = x.f;
         gf[c] = g.f;
 #pragma unroll
-        for (int i = 0; i < AT::E; i++) delta += (float)g.f[i] * (float)o.f[i];
+        for (int i = 0; i < AT::E; i++) delta += (float)g.f[i] * ((float)o.f[i] + (float)e.f[i]);
     }
     delta += other_half(delta);
-    const int64_t stat = ((int64_t)b * p.hq + h) * p.sq + row;
-    float lse = kInf;                                              // a row that sees nothing, or is none: every p is zero
+    // the statistics of this tile's rows, for both kernels; a row that sees nothing, or is none, has every p zero
+    float lse = kInf;
     if (live) {
-        const float x = p.lse[stat];
+        const float x = p.lse[((int64_t)b * p.hq + h) * p.sq + row];
         lse = x == -kInf ? kInf : x * kScoreUnit;
-        if (half == 0) p.delta[stat] = delta;
+    }
+    if (half == 0) {
+        float *st = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad + row;
+        st[0] = lse;
+        st[p.sq_pad] = delta;
     }
 
-    int dq_id = 0, w_lo = 0, w_hi = 0;
-    int2 wg_span = {0, 0};
-    const int *docs = p.docs != nullptr ? p.docs + b * p.docs_b : nullptr;
+    int id = 0;
+    int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
-    if (threadIdx.x == 0) lds_bad = -1;
-    if (docs != nullptr) {
-        const int raw = live ? max(docs[pos], -1) : -1;
-        w_lo = wave_min(raw);
-        w_hi = wave_max(raw);
-        if (lane == 0) { lds_doc[wave] = w_lo; lds_doc[4 + wave] = w_hi; }
-        dq_id = raw < 0 ? -2 : raw;
+    const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
+    if (p.docs != nullptr) {
+        const int raw = live ? ids[pos] : -1;
+        span = {wave_min(raw), wave_max(raw)};
+        if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
+        id = raw < 0 ? -2 : raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
     }
     const int key_end = p.causal ? max(min(pos_end, p.sk), prefix) : p.sk;
-    const int tiles = key_end > 0 ? (key_end + TK - 1) / TK : 0;
+    TileWalk walk;
+    walk.start(0, key_end > 0 ? (key_end + TK - 1) / TK : 0);
+    const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
+        const int k0 = t * TK, k1 = k0 + TK;
+        const bool inside = k1 <= p.sk, in_prefix = !p.causal || k1 <= prefix;
+        whole = inside && (in_prefix || k1 - 1 <= i0 + off);
+        full = inside && (in_prefix || k1 - 1 <= pos_lo);
+        skip = p.causal && k0 > pos_lo + 31 && k0 >= prefix;
+        if (p.docs != nullptr) {
+            const int2 s = doc_span(ranges, k0, min(k1, p.sk));
+            want = docs_meet(s, wg_span);
+            whole = whole && docs_same(s, wg_span);
+            full = full && docs_same(s, span);
+            skip = skip || !docs_meet(s, span);
+        }
+    };
 
     fx16 acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) acc[db] = fx16{};
-    float dslope = 0.f;
+    // sum_j dS |dist|, sum_j dS and sum_j P |dist|: the second is what the rounding of out left in delta, and is taken out
+    float far = 0.f, left = 0.f, reach = 0.f;
+    const float unit = p.scale * kScoreUnit;
 
-    for (int base = 0; base < tiles; base += 64) {
-        bool want = base + lane < tiles;
-        if (docs != nullptr && want) {
-            const int k0 = (base + lane) * TK;
-            want = docs_meet(doc_span(ranges, k0, min(k0 + TK, p.sk)), wg_span);
+    int buf = 0, tile = walk.next(look);
+    bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
+    if (tile >= 0) {
+        feed_k.issue(lds, tile * TK, min(TK, p.sk - tile * TK));
+        feed_v.issue(lds + kTileBytes, tile * TK, min(TK, p.sk - tile * TK));
+    }
+    while (tile >= 0) {
+        const int k0 = tile * TK;
+        char *lds_k = lds + buf * 2 * kTileBytes, *lds_v = lds_k + kTileBytes;
+        const int next = walk.next(look);
+        FD::wait();
+        __syncthreads();
+        buf ^= 1;
+        if (next >= 0) {
+            feed_k.issue(lds + buf * 2 * kTileBytes, next * TK, min(TK, p.sk - next * TK));
+            feed_v.issue(lds + buf * 2 * kTileBytes + kTileBytes, next * TK, min(TK, p.sk - next * TK));
         }
-        for (uint64_t todo = __ballot(want); todo != 0; todo &= todo - 1) {
-            const int tile = base + __builtin_ctzll(todo), k0 = tile * TK, rows = min(TK, p.sk - k0);
-            bool doc_full = true, wave_doc_full = true;
-            if (docs != nullptr) {
-                const int2 s = doc_span(ranges, k0, k0 + rows);
-                doc_full = s.x == s.y && s.x >= 0 && wg_span.x == s.x && wg_span.y == s.x;
-                wave_doc_full = s.x == s.y && s.x >= 0 && w_lo == s.x && w_hi == s.x;
-            }
-            const bool in_prefix = k0 + TK <= prefix;
-            const bool whole = rows == TK && doc_full && (!p.causal || in_prefix || k0 + TK - 1 <= i0 + off);
-            const bool full = rows == TK && wave_doc_full && (!p.causal || in_prefix || k0 + TK - 1 <= pos_lo);
-            Stage<T, DP, TK> sk, sv;
-            sk.load(kbase + (int64_t)k0 * p.ks.s, p.ks.s, rows, p.d, p.vec);
-            sv.load(vbase + (int64_t)k0 * p.vs.s, p.vs.s, rows, p.dv_d, p.vec);
+        if (!whole) {                                              // a row that sees what this removes has a lse of NaN
+            FD::clean_share(lds_k);
             __syncthreads();
-            sk.store(lds_k);
-            sv.store(lds_v);
-            if (!whole && sk.nonfinite()) lds_bad = tile;
-            __syncthreads();
-            const bool careful = !whole && lds_bad == tile;
-            if (p.causal && k0 > pos_lo + 31 && k0 >= prefix) continue;
+        }
+        if (!skip) {
+            const int lim = last - k0 - 4 * half;
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 fx16 s = {}, dp = {};
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    s = AT::mma(TL::rows(lds_k, 32 * kb, c), qf[c], s);
-                    dp = AT::mma(TL::rows(lds_v, 32 * kb, c), gf[c], dp);
+                    s = AT::mma(TL::rows(lds_k, at_lane, 32 * kb, c), qf[c], s);
+                    dp = AT::mma(TL::rows(lds_v, at_lane, 32 * kb, c), gf[c], dp);
+                }
+                bool hide[16];
+                if (!full) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) hide[r] = 32 * kb + 8 * (r >> 2) + (r & 3) > lim;
+                    if (p.docs != nullptr) {
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            const int4 t = *(const int4 *)(ids + min(k0 + 32 * kb, (p.doc_blocks - 1) * kDocBlock) + 8 * g + 4 * half);
+                            hide[4 * g] |= t.x != id;
+                            hide[4 * g + 1] |= t.y != id;
+                            hide[4 * g + 2] |= t.z != id;
+                            hide[4 * g + 3] |= t.w != id;
+                        }
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3);
-                    float t = 0.f;
-                    const float x = score<T, MOD>(p, s[r], slope, pos, key, t);
-                    float g = __builtin_amdgcn_exp2f(x - lse) * (dp[r] - delta);
-                    bool see = live;
-                    if (!full) {
-                        see = see && key < p.sk && (!p.causal || key <= pos || key < prefix);
-                        if (docs != nullptr) see = see && docs[min(key, p.sk - 1)] == dq_id;
-                    }
-                    g = see ? g : 0.f;
-                    if (MOD) {
-                        dslope -= g * __builtin_fabsf((float)(pos - key));
+                    float e, g, t = 0.f;
+                    if constexpr (MOD) {
+                        const int dist = pos - (k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3));
+                        e = __builtin_amdgcn_exp2f(score<T>(p, s[r], slope, dist, t) - lse);
+                        g = e * (dp[r] - delta);
+                        if (!full) { e = hide[r] ? 0.f : e; g = hide[r] ? 0.f : g; }
+                        if (p.dslopes_part != nullptr) {
+                            const float a = __builtin_fabsf((float)dist);
+                            far += g * a;
+                            left += g;
+                            reach += e * a;
+                        }
                         if (p.cap > 0.f) g *= 1.f - t * t;
+                    } else {
+                        e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit, -lse));
+                        g = e * (dp[r] - delta);
+                        if (!full) g = hide[r] ? 0.f : g;
                     }
                     s[r] = g;
                 }
@@ -145,19 +183,23 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_dq_kernel(AttnArgs 
                 for (int st = 0; st < ST; st++) {
                     const frag gfr = pack<T>(s, st);
 #pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        const frag kf = TL::cols(lds_k, 32 * kb + AT::KS * st, 32 * db);
-                        if (careful) acc[db] = mma_careful<T>(kf, gfr, acc[db]);
-                        else acc[db] = AT::mma(kf, gfr, acc[db]);
-                    }
+                    for (int db = 0; db < DB; db++) acc[db] = AT::mma(TL::cols(lds_k, at_lane, 32 * kb + AT::KS * st, db), gfr, acc[db]);
                 }
             }
         }
+        tile = next;
+        whole = walk.is_whole;
+        full = walk.is_full;
+        skip = walk.is_skip;
     }
     if (MOD && p.dslopes_part != nullptr) {                        // in a fixed order: lanes, then waves
+        far += other_half(far);
+        left += other_half(left);
+        reach += other_half(reach);
+        float x = live && half == 0 ? left * reach - far : 0.f;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) dslope += __shfl_xor(dslope, o, 64);
-        if (lane == 0) lds_sum[wave] = dslope;
+        for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+        if (lane == 0) lds_sum[wave] = x;
         __syncthreads();
         if (threadIdx.x == 0)
             p.dslopes_part[((int64_t)h * p.b + b) * tiles_q + tile_q] = (lds_sum[0] + lds_sum[1]) + (lds_sum[2] + lds_sum[3]);
@@ -179,25 +221,27 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
     constexpr int TQ = AT::kTile, QB = TQ / 32, C = DP / AT::KS, DB = DP / 32, ST = 32 / AT::KS;
-    __shared__ __align__(16) char lds_q[TQ * TL::RB];
-    __shared__ __align__(16) char lds_g[TQ * TL::RB];
-    __shared__ float lds_lse[TQ], lds_delta[TQ];
-    __shared__ int lds_id[TQ];
+    typedef Feed<T, DP, TQ> FD;
+    constexpr int kTileBytes = TQ * TL::RB;
+    __shared__ __align__(16) char lds[4 * kTileBytes];
+    __shared__ __align__(16) float lds_stat[2][2][TQ];             // lse and delta of a tile's rows
+    __shared__ __align__(16) int lds_id[2][TQ];
     __shared__ int lds_doc[8];
-    __shared__ int lds_bad;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int pairs = p.b * p.hk, tiles_k = (p.sk + kAttnRows - 1) / kAttnRows;
     const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs % p.splits, tile_k = blockIdx.x / pairs / p.splits;
     const int b = pair / p.hk, hk = pair % p.hk;
     const int off = p.sk - p.sq;
-    const int k0 = tile_k * kAttnRows, key = k0 + wave * 32 + (lane & 31);
+    const int k0 = tile_k * kAttnRows, k_lo = k0 + wave * 32, key = k_lo + (lane & 31);
     const bool live = key < p.sk;
-    const int k_lo = k0 + wave * 32;
     const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int first = p.causal && key >= prefix ? key - off : 0;   // first row that sees this key
 
     const T *krow = (const T *)p.k + b * p.ks.b + hk * p.ks.h + (int64_t)key * p.ks.s;
     const T *vrow = (const T *)p.v + b * p.vs.b + hk * p.vs.h + (int64_t)key * p.vs.s;
+    typename TL::Lane at_lane;
+    at_lane.init();
     frag kf[C], vf[C];
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -207,114 +251,143 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
         kf[c] = x.f;
         vf[c] = y.f;
     }
-    int key_id = 0, w_lo = 0, w_hi = 0;
-    int2 wg_span = {0, 0};
-    const int *docs = p.docs != nullptr ? p.docs + b * p.docs_b : nullptr;
+    int id = 0;
+    int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
-    if (threadIdx.x == 0) lds_bad = -1;
-    if (docs != nullptr) {
-        const int raw = live ? max(docs[key], -1) : -1;
-        w_lo = wave_min(raw);
-        w_hi = wave_max(raw);
-        if (lane == 0) { lds_doc[wave] = w_lo; lds_doc[4 + wave] = w_hi; }
-        key_id = raw < 0 ? -2 : raw;
+    const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
+    if (p.docs != nullptr) {
+        const int raw = live ? ids[key] : -1;
+        span = {wave_min(raw), wave_max(raw)};
+        if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
+        id = raw < 0 ? -2 : raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
     }
-    // rows that may see a key of this tile: with the causal mask those at or behind its first key, or all for a prefix
-    const int first = p.causal && k0 >= prefix ? max(k0 - off, 0) : 0;
-    const int tile_lo = first / TQ, tile_hi = (p.sq + TQ - 1) / TQ;
+    // rows that may see a key of this tile: with the causal mask those at or behind its first key, or all for a prefix.
+    // A row past the last one has statistics that make its weights zero, and needs no mask.
+    const int lo = p.causal && k0 >= prefix ? max(k0 - off, 0) : 0;
+    const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
+        const int i0 = t * TQ, i1 = min(i0 + TQ, p.sq);
+        whole = !p.causal || k0 + kAttnRows - 1 <= i0 + off || k0 + kAttnRows <= prefix;
+        full = !p.causal || k_lo + 31 <= i0 + off || k_lo + 32 <= prefix;
+        skip = p.causal && k_lo > i0 + TQ - 1 + off && k_lo >= prefix;
+        if (p.docs != nullptr) {
+            const int2 s = doc_span(ranges, i0 + off, i1 + off);
+            want = docs_meet(s, wg_span);
+            whole = whole && docs_same(s, wg_span);
+            full = full && docs_same(s, span);
+            skip = skip || !docs_meet(s, span);
+        }
+    };
 
     fx16 dk[DB], dv[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
+    const float unit = p.scale * kScoreUnit;
 
     const int h_lo = p.group * split / p.splits, h_hi = p.group * (split + 1) / p.splits;
     for (int hg = h_lo; hg < h_hi; hg++) {
         const int h = hk * p.group + hg;
         const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
-        const T *qbase = (const T *)p.q + b * p.qs.b + h * p.qs.h;
-        const T *gbase = (const T *)p.dout + b * p.dos.b + h * p.dos.h;
-        const int64_t stat = ((int64_t)b * p.hq + h) * p.sq;
-        for (int base = tile_lo; base < tile_hi; base += 64) {
-            bool want = base + lane < tile_hi;
-            if (docs != nullptr && want) {
-                const int lo = (base + lane) * TQ;
-                want = docs_meet(doc_span(ranges, lo + off, min(lo + TQ, p.sq) + off), wg_span);
+        const float *stats = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad;
+        FD feed_q, feed_g;
+        feed_q.init((const T *)p.q + b * p.qs.b + h * p.qs.h, p.qs.s, p.d, p.vec);
+        feed_g.init((const T *)p.dout + b * p.dos.b + h * p.dos.h, p.dos.s, p.dv_d, p.vec);
+        // a tile's statistics (padded to whole tiles of 128 rows) and ids pass through registers of its first threads
+        float r_lse = 0.f, r_delta = 0.f;
+        int r_id = -1;
+        const bool mine = (int)threadIdx.x < TQ;
+        const auto issue = [&](int t, char *to) {
+            const int i0 = t * TQ, rows = min(TQ, p.sq - i0);
+            feed_q.issue(to, i0, rows);
+            feed_g.issue(to + kTileBytes, i0, rows);
+            if (mine) {
+                r_lse = stats[i0 + threadIdx.x];
+                r_delta = stats[p.sq_pad + i0 + threadIdx.x];
+                if (p.docs != nullptr) r_id = (int)threadIdx.x < rows ? ids[i0 + off + threadIdx.x] : -1;
             }
-            for (uint64_t todo = __ballot(want); todo != 0; todo &= todo - 1) {
-                const int tile = base + __builtin_ctzll(todo), i0 = tile * TQ, rows = min(TQ, p.sq - i0);
-                bool doc_full = true, wave_doc_full = true;
-                if (docs != nullptr) {
-                    const int2 s = doc_span(ranges, i0 + off, i0 + rows + off);
-                    doc_full = s.x == s.y && s.x >= 0 && wg_span.x == s.x && wg_span.y == s.x;
-                    wave_doc_full = s.x == s.y && s.x >= 0 && w_lo == s.x && w_hi == s.x;
-                }
-                const bool whole = rows == TQ && doc_full && (!p.causal || k0 + kAttnRows - 1 <= i0 + off || k0 + kAttnRows <= prefix);
-                const bool full = rows == TQ && wave_doc_full && (!p.causal || k_lo + 31 <= i0 + off || k_lo + 32 <= prefix);
-                Stage<T, DP, TQ> sq, sg;
-                sq.load(qbase + (int64_t)i0 * p.qs.s, p.qs.s, rows, p.d, p.vec);
-                sg.load(gbase + (int64_t)i0 * p.dos.s, p.dos.s, rows, p.dv_d, p.vec);
-                float r_lse = kInf, r_delta = 0.f;
-                int r_id = -1;
-                if ((int)threadIdx.x < rows) {
-                    const float x = p.lse[stat + i0 + threadIdx.x];
-                    r_lse = x == -kInf ? kInf : x * kScoreUnit;
-                    r_delta = p.delta[stat + i0 + threadIdx.x];
-                    if (docs != nullptr) r_id = max(docs[i0 + threadIdx.x + off], -1);
-                }
+        };
+        const auto put = [&](int to) {
+            if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; lds_id[to][threadIdx.x] = r_id; }
+        };
+        TileWalk walk;
+        walk.start(lo / TQ, (p.sq + TQ - 1) / TQ);
+        int buf = 0, tile = walk.next(look);
+        bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
+        __syncthreads();                                           // the tiles of the head before have been read
+        if (tile >= 0) { issue(tile, lds); put(0); }
+        while (tile >= 0) {
+            const int i0 = tile * TQ;
+            char *lds_q = lds + buf * 2 * kTileBytes, *lds_g = lds_q + kTileBytes;
+            const float *lse_of = lds_stat[buf][0], *delta_of = lds_stat[buf][1];
+            const int *id_of = lds_id[buf];
+            const int next = walk.next(look);
+            FD::wait();
+            __syncthreads();
+            buf ^= 1;
+            if (next >= 0) issue(next, lds + buf * 2 * kTileBytes);
+            if (!whole) {                                          // a bad row of q has a lse of NaN, one of dout a delta
+                FD::clean_share(lds_q);
+                FD::clean_share(lds_g);
                 __syncthreads();
-                sq.store(lds_q);
-                sg.store(lds_g);
-                if (threadIdx.x < TQ) { lds_lse[threadIdx.x] = r_lse; lds_delta[threadIdx.x] = r_delta; lds_id[threadIdx.x] = r_id; }
-                const int seq = hg * tile_hi + tile;
-                if (!whole && (sq.nonfinite() || sg.nonfinite())) lds_bad = seq;
-                __syncthreads();
-                const bool careful = !whole && lds_bad == seq;
-                if (p.causal && k_lo > i0 + TQ - 1 + off && k_lo >= prefix) continue;
+            }
+            if (!skip) {
+                const int lim = first - i0 - 4 * half;
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++) {
                     fx16 s = {}, dp = {};
 #pragma unroll
                     for (int c = 0; c < C; c++) {
-                        s = AT::mma(TL::rows(lds_q, 32 * qb, c), kf[c], s);
-                        dp = AT::mma(TL::rows(lds_g, 32 * qb, c), vf[c], dp);
+                        s = AT::mma(TL::rows(lds_q, at_lane, 32 * qb, c), kf[c], s);
+                        dp = AT::mma(TL::rows(lds_g, at_lane, 32 * qb, c), vf[c], dp);
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int at = 32 * qb + 8 * (r >> 2) + 4 * half + (r & 3), i = i0 + at, pos = i + off;
-                        float t = 0.f;
-                        const float x = score<T, MOD>(p, s[r], slope, pos, key, t);
-                        float e = __builtin_amdgcn_exp2f(x - lds_lse[at]);
-                        float g = e * (dp[r] - lds_delta[at]);
-                        bool see = live;
+                    for (int g4 = 0; g4 < 4; g4++) {
+                        const int a = 32 * qb + 8 * g4 + 4 * half;
+                        const fx4 lse = *(const fx4 *)(lse_of + a), delta = *(const fx4 *)(delta_of + a);
+                        bool hide[4];
                         if (!full) {
-                            see = see && i < p.sq && (!p.causal || key <= pos || key < prefix);
-                            if (docs != nullptr) see = see && lds_id[at] == key_id;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) hide[i] = 32 * qb + 8 * g4 + i < lim;
+                            if (p.docs != nullptr) {
+                                const int4 t = *(const int4 *)(id_of + a);
+                                hide[0] |= t.x != id;
+                                hide[1] |= t.y != id;
+                                hide[2] |= t.z != id;
+                                hide[3] |= t.w != id;
+                            }
                         }
-                        if (MOD && p.cap > 0.f) g *= 1.f - t * t;
-                        s[r] = see ? e : 0.f;
-                        dp[r] = see ? g : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = 4 * g4 + i;
+                            float e, g, t = 0.f;
+                            if constexpr (MOD) e = __builtin_amdgcn_exp2f(score<T>(p, s[r], slope, i0 + a + i + off - key, t) - lse[i]);
+                            else e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit, -lse[i]));
+                            g = e * (dp[r] - delta[i]);
+                            if (MOD && p.cap > 0.f) g *= 1.f - t * t;
+                            if (!whole) e = __builtin_fmaf(delta[i], 0.f, e);
+                            if (!full) { e = hide[i] ? 0.f : e; g = hide[i] ? 0.f : g; }
+                            s[r] = e;
+                            dp[r] = g;
+                        }
                     }
 #pragma unroll
                     for (int st = 0; st < ST; st++) {
                         const frag pf = pack<T>(s, st), sf = pack<T>(dp, st);
 #pragma unroll
                         for (int db = 0; db < DB; db++) {
-                            const frag gt = TL::cols(lds_g, 32 * qb + AT::KS * st, 32 * db);
-                            const frag qt = TL::cols(lds_q, 32 * qb + AT::KS * st, 32 * db);
-                            if (careful) {
-                                dv[db] = mma_careful<T>(gt, pf, dv[db]);
-                                dk[db] = mma_careful<T>(qt, sf, dk[db]);
-                            } else {
-                                dv[db] = AT::mma(gt, pf, dv[db]);
-                                dk[db] = AT::mma(qt, sf, dk[db]);
-                            }
+                            dv[db] = AT::mma(TL::cols(lds_g, at_lane, 32 * qb + AT::KS * st, db), pf, dv[db]);
+                            dk[db] = AT::mma(TL::cols(lds_q, at_lane, 32 * qb + AT::KS * st, db), sf, dk[db]);
                         }
                     }
                 }
             }
+            if (next >= 0) put(buf);
+            tile = next;
+            whole = walk.is_whole;
+            full = walk.is_full;
+            skip = walk.is_skip;
         }
     }
     if (!live) return;

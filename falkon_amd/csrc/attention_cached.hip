@@ -39,6 +39,8 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const T *kbase = (const T *)p.k + b * p.ks.b + hk * p.ks.h;
     const T *vbase = (const T *)p.v + b * p.vs.b + hk * p.vs.h;
     char *lds_k = lds + wave * kLds, *lds_v = lds_k + TK * TL::RB;
+    typename TL::Lane at_lane;
+    at_lane.init();
     frag qf[C];
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         if (tile + 4 < tile_hi) fetch(tile + 4);
         fx16 s = {};
 #pragma unroll
-        for (int c = 0; c < C; c++) s = AT::mma(TL::rows(lds_k, 0, c), qf[c], s);
+        for (int c = 0; c < C; c++) s = AT::mma(TL::rows(lds_k, at_lane, 0, c), qf[c], s);
         float top = -kInf;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -107,15 +109,32 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         }
         const float base_m = m == -kInf ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < 16; i++) { s[i] = __builtin_amdgcn_exp2f(s[i] - base_m); l += s[i]; }
+        for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(s[i] - base_m);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};                       // short chains: long ones would cost float data digits
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum[i & 3] += s[i];
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (careful) {
+            fx16 w = s, x[DB];                                     // through copies, so that s and o stay in registers elsewhere
+#pragma unroll
+            for (int db = 0; db < DB; db++) x[db] = o[db];
+            spread_nonfinite<T, DP, 1, DB>(lds_v, &w, x);
+#pragma unroll
+            for (int db = 0; db < DB; db++) o[db] = x[db];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int n = 0; n < N; n++) clean<T>(lds_v + (n * 64 + lane) * 16);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
         for (int st = 0; st < ST; st++) {
             const frag pf = pack<T>(s, st);
 #pragma unroll
             for (int db = 0; db < DB; db++) {
-                const frag vf = TL::cols(lds_v, AT::KS * st, 32 * db);
-                if (careful) o[db] = mma_careful<T>(vf, pf, o[db]);
-                else o[db] = AT::mma(vf, pf, o[db]);
+                const frag vf = TL::cols(lds_v, at_lane, AT::KS * st, db);
+                o[db] = AT::mma(vf, pf, o[db]);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

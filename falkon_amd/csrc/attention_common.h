@@ -79,30 +79,42 @@ template <typename T, int DP> struct Tile {
     static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
 
     typedef typename AttnType<T>::frag frag;
-    // step c of the row of this lane (row0 + lane % 32)
-    static __device__ __forceinline__ frag rows(const char *tile, int row0, int c) {
-        const int l = threadIdx.x & 63;
-        return *(const frag *)(tile + at(row0 + (l & 31), 2 * c + (l >> 5)));
+    // This lane's places in a tile.  Only the low bits of a chunk's number are permuted, so a handful of offsets and
+    // constants on top of them reach every fragment.
+    static constexpr int RV = RB % 128 == 0 ? 4 : 2, CV = sizeof(T) == 4 ? 4 : RB % 128 == 0 ? 2 : 1;
+    struct Lane {
+        int r[RV], c[CV];
+        __device__ __forceinline__ void init() {
+            const int l = threadIdx.x & 63, h = l >> 5, m = l & 31;
+#pragma unroll
+            for (int x = 0; x < RV; x++) r[x] = at(m, 2 * x + h);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) c[x] = at(4 * h + x, m >> 2) + (m & 3) * 4;
+            } else {
+                // the transposing read: of 16 lanes, four each name 4 values of one row; lane i gets column i of the four rows
+#pragma unroll
+                for (int x = 0; x < CV; x++) c[x] = at(4 * h + (l >> 2 & 3), 4 * x + 2 * (l >> 4 & 1) + (l >> 1 & 1)) + (l & 1) * 8;
+            }
+        }
+    };
+    // step c of the row of this lane (row0 + lane % 32; row0 a multiple of 32)
+    static __device__ __forceinline__ frag rows(const char *tile, const Lane &p, int row0, int c) {
+        return *(const frag *)(tile + p.r[c % RV] + row0 * RB + c / RV * RV * 32);
     }
-    // columns d0 + lane % 32 of KS rows from row0 on, in the order in which the accumulator registers hold rows
-    static __device__ __forceinline__ frag cols(const char *tile, int row0, int d0) {
-        const int l = threadIdx.x & 63, h = l >> 5;
+    // columns 32 db + lane % 32 of KS rows from row0 on (a multiple of KS), in the order in which the accumulator registers
+    // hold rows
+    static __device__ __forceinline__ frag cols(const char *tile, const Lane &p, int row0, int db) {
         frag f;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int c = d0 + (l & 31);
-                f[i] = *(const float *)(tile + at(row0 + 4 * h + i, c >> 2) + (c & 3) * 4);
-            }
+            for (int i = 0; i < 4; i++) f[i] = *(const float *)(tile + p.c[i] + row0 * RB + db * 128);
         } else {
-            // the transposing read: of 16 lanes, four each name 4 values of one row; lane i gets column i of the four rows
-            const int i = l & 15, b = (d0 + (l & 16)) * 2 + (i & 3) * 8;
             union { sx4 s[2]; frag f; } u;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const char *p = tile + at(row0 + 8 * k + 4 * h + (i >> 2), b >> 4) + (b & 8);
-                u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4 *)p);
-            }
+            for (int k = 0; k < 2; k++)
+                u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) sx4 *)(tile + p.c[db % CV] + (row0 + 8 * k) * RB + db / CV * CV * 64));
             f = u.f;
         }
         return f;
@@ -120,45 +132,55 @@ template <typename T> __device__ __forceinline__ typename AttnType<T>::frag pack
     return f;
 }
 
-// Product with rows that may hold infinities or NaNs in places this step's weights hide: those get no share, and where a
-// weight that is not zero meets one, the sum becomes what the formula gives.
-template <typename T>
-__device__ __forceinline__ fx16 mma_careful(typename AttnType<T>::frag a, typename AttnType<T>::frag p, fx16 c) {
-    typename AttnType<T>::frag up = a, down = a, seen = p;
+// Infinities and NaNs of a tile must not reach rows that hide them, but a product with weight zero would carry them there.
+// They are set to zero in LDS where a mask is needed; clean() does it to this thread's 16 bytes.
+template <typename T> __device__ __forceinline__ bool any_nonfinite(ux4 u);
+template <typename T> __device__ __forceinline__ void clean(char *at) {
+    union { ux4 u; T t[16 / sizeof(T)]; } x;
+    x.u = *(const ux4 *)at;
+    if (!any_nonfinite<T>(x.u)) return;
 #pragma unroll
-    for (int i = 0; i < AttnType<T>::E; i++) {
-        const float x = (float)a[i];
-        const bool fine = __builtin_fabsf(x) < kInf;
-        up[i] = (T)(fine || x == -kInf ? 0.f : 1.f);
-        down[i] = (T)(fine || x == kInf ? 0.f : 1.f);
-        seen[i] = (T)((float)p[i] == 0.f ? 0.f : 1.f);
-        if (!fine) a[i] = (T)0.f;
+    for (int i = 0; i < (int)(16 / sizeof(T)); i++)
+        if (!(__builtin_fabsf((float)x.t[i]) < kInf)) x.t[i] = (T)0.f;
+    *(ux4 *)at = x.u;
+}
+// What they add to the rows that see them: value (row, c) of a tile of TK rows for every output column this lane holds, where the
+// row's weight is not zero.  w[kb][r]: weights of key 32 kb + 8 (r / 4) + 4 half + r % 4.  Rare, and not made to be fast.
+template <typename T, int DP, int KB, int DB>
+__device__ __noinline__ void spread_nonfinite(const char *tile, const fx16 *w, fx16 *o) {
+    typedef Tile<T, DP> TL;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    for (int key = 0; key < 32 * KB; key++) {
+        const ux4 mine = lane < TL::NC ? *(const ux4 *)(tile + TL::at(key, lane)) : ux4{0, 0, 0, 0};
+        if (!__any(any_nonfinite<T>(mine))) continue;
+        float x = w[key >> 5][4 * (key >> 3 & 3) + (key & 3)];
+        const float y = __shfl_xor(x, 32, 64);
+        x = (key >> 2 & 1) == half ? x : y;
+        for (int db = 0; db < DB; db++)
+            for (int r = 0; r < 16; r++) {
+                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
+                const float v = (float)*(const T *)(tile + TL::at(key, c / AttnType<T>::E) + c % AttnType<T>::E * (int)sizeof(T));
+                if (x != 0.f && !(__builtin_fabsf(v) < kInf)) o[db][r] += v;
+            }
     }
-    fx16 u = {}, d = {};
-    c = AttnType<T>::mma(a, p, c);
-    u = AttnType<T>::mma(up, seen, u);
-    d = AttnType<T>::mma(down, seen, d);
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if (u[i] > 0.f) c[i] += kInf;
-        if (d[i] > 0.f) c[i] -= kInf;
-    }
-    return c;
 }
 
 struct AttnStride { int64_t b, s, h; };
 struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
-    void *o, *dq, *dk, *dv;
-    float *lse, *delta, *dslopes_part, *dkv_part;
-    AttnStride qs, ks, vs, os, dos;                    // strides of q, k, v, out and dout; the gradients are contiguous
+    void *o, *rest, *dq, *dk, *dv;                     // rest: what rounding took from out, for the backward pass
+    float *lse, *dslopes_part, *dkv_part;
+    float *stats;                                      // backward: [b][hq][2][sq_pad], the rows' lse (in units of log 2) and delta
+    int64_t sq_pad;
+    AttnStride qs, ks, vs, dos;                        // strides of q, k, v and dout; the others are contiguous
     int b, sq, sk, hq, hk, group, d, dv_d;
     int splits;                                        // dk / dv: parts the heads of a group are divided into
     float scale, cap;
     const float *slopes;
     const int *prefix, *docs;
     int64_t docs_b;
-    int2 *doc_range;                                   // [b][blocks of kDocBlock positions]
+    int2 *doc_range;                                   // [b][doc_blocks]: smallest and largest id of kDocBlock positions
+    int *doc_ids;                                      // [b][doc_blocks * kDocBlock]: the ids, -1 for padding and past the end
     int doc_blocks;
     int causal, vec;                                   // vec: all rows can be read 16 bytes at a time
 };
@@ -181,28 +203,66 @@ template <typename T> __device__ __forceinline__ ux4 load_chunk(const T *row, in
     return r;
 }
 
-// The share of this thread in a tile of TR rows: global memory to registers, later registers to LDS.
-template <typename T, int DP, int TR> struct Stage {
-    static constexpr int NC = Tile<T, DP>::NC, N = (TR * NC + kAttnThreads - 1) / kAttnThreads;
-    ux4 r[N];
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int rows, int d, int vec) {
+// Tiles of TR rows on their way into LDS.  Aligned rows go there directly, 16 bytes a lane, without passing through registers:
+// a wave's instruction fills 1024 consecutive bytes of LDS, so the permutation of the chunks is applied to the addresses
+// read.  Lanes past the last row or the row's end read out of the buffer's bounds and bring zeros.  The reads are counted by
+// vmcnt; wait() and a barrier stand between them and the tile's use.  Their targets are named by 16 bits, so tiles lie in the first
+// 64 KB of LDS.  Other rows are read value by value.
+constexpr unsigned kNowhere = 0x80000000u;                 // an offset behind every buffer's end
+template <typename T, int DP, int TR> struct Feed {
+    typedef Tile<T, DP> TL;
+    static constexpr int NC = TL::NC, N = TR * NC / kAttnThreads, kStep = kAttnThreads / NC;
+    static_assert(TR * NC % kAttnThreads == 0, "every instruction is full");
+    static constexpr bool kEven = kAttnThreads % NC == 0 && kStep % 8 == 0;   // all instructions permute alike
+    const T *base;
+    int64_t stride;
+    unsigned off[kEven ? 1 : N];
+    int d, vec;
+    __device__ __forceinline__ void init(const T *b, int64_t st, int d_, int vec_) {
+        base = b; stride = st; d = d_; vec = vec_;
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int i = n * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC;
-            r[n] = load_chunk<T>(base + row * stride, c, d, row < rows && i < TR * NC, vec);
+        for (int n = 0; n < (kEven ? 1 : N); n++) {
+            const int i = n * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC ^ TL::swz(row);
+            off[n] = c * AttnType<T>::E < d ? (unsigned)(row * (int)(stride * sizeof(T)) + c * 16) : kNowhere;
         }
     }
-    __device__ __forceinline__ void store(char *tile) const {
+    __device__ __forceinline__ void issue(char *tile, int row0, int rows) const {
+        if (vec) {
+            const uint64_t a = (uint64_t)(base + row0 * stride);
+            ux4 rsrc;
+            rsrc[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+            rsrc[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu);
+            rsrc[2] = 0x7fffffffu;
+            rsrc[3] = 0x00027000u;
+            const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)tile +
+                                                               (threadIdx.x & ~63u) * 16);
+            const int step = __builtin_amdgcn_readfirstlane((int)(kStep * stride * sizeof(T)));
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int i = n * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC;
-            if (TR * NC % kAttnThreads == 0 || i < TR * NC) *(ux4 *)(tile + Tile<T, DP>::at(row, c)) = r[n];
+            for (int n = 0; n < N; n++) {
+                unsigned o = off[kEven ? 0 : n];
+                if (rows < TR && (n * kAttnThreads + (int)threadIdx.x) / NC >= rows) o = kNowhere;
+                const int so = kEven ? n * step : 0;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                             :: "s"(to + n * kAttnThreads * 16), "v"(o), "s"(rsrc), "s"(so) : "memory", "m0");
+            }
+        } else {
+#pragma unroll 1
+            for (int n = 0; n < N; n++) {
+                const int i = n * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC;
+                *(ux4 *)(tile + TL::at(row, c)) = load_chunk<T>(base + (row0 + row) * stride, c, d, row < rows, 0);
+            }
         }
     }
-    __device__ __forceinline__ bool nonfinite() const {
+    static __device__ __forceinline__ void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    static __device__ __forceinline__ void clean_share(char *tile) {
+#pragma unroll
+        for (int n = 0; n < N; n++) clean<T>(tile + (n * kAttnThreads + threadIdx.x) * 16);
+    }
+    // whether this thread's share of a tile in LDS holds an infinity or a NaN
+    static __device__ __forceinline__ bool nonfinite(const char *tile) {
         bool bad = false;
 #pragma unroll
-        for (int n = 0; n < N; n++) bad |= any_nonfinite<T>(r[n]);
+        for (int n = 0; n < N; n++) bad |= any_nonfinite<T>(*(const ux4 *)(tile + (n * kAttnThreads + threadIdx.x) * 16));
         return bad;
     }
 };
@@ -218,12 +278,11 @@ template <typename T> __device__ __forceinline__ float tanh_of(float u) {
 }
 
 // One score in units of log 2, and the tanh (for its derivative)
-template <typename T, bool MOD>
-__device__ __forceinline__ float score(const AttnArgs &p, float s, float slope, int pos, int key, float &t) {
-    if constexpr (!MOD) return s * (p.scale * kScoreUnit);
+template <typename T>
+__device__ __forceinline__ float score(const AttnArgs &p, float s, float slope, int dist, float &t) {
     float x = s * p.scale;
     if (p.cap > 0.f) { t = tanh_of<T>(x * __builtin_amdgcn_rcpf(p.cap)); x = p.cap * t; }
-    return (x - slope * __builtin_fabsf((float)(pos - key))) * kScoreUnit;
+    return (x - slope * __builtin_fabsf((float)dist)) * kScoreUnit;
 }
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
@@ -245,6 +304,35 @@ __device__ __forceinline__ int2 doc_span(const int2 *range, int lo, int hi) {
     return s;
 }
 __device__ __forceinline__ bool docs_meet(int2 a, int2 b) { return a.y >= 0 && b.y >= 0 && a.x <= b.y && b.x <= a.y; }
+__device__ __forceinline__ bool docs_same(int2 a, int2 b) { return a.x >= 0 && a.x == a.y && a.x == b.x && a.x == b.y; }
+
+// The tiles a workgroup visits, in rising order, 64 at a time: lane t looks at tile base + t.  `whole`: no row of the
+// workgroup needs a mask there; `full`, `skip`: this wave's rows need none, or see nothing.
+struct TileWalk {
+    int base, end;
+    uint64_t todo, whole, full, skip;
+    bool is_whole, is_full, is_skip;
+    __device__ __forceinline__ void start(int lo, int hi) { base = lo - 64; end = hi; todo = 0; }
+    template <typename Look> __device__ __forceinline__ int next(Look look) {
+        while (todo == 0) {
+            base += 64;
+            if (base >= end) return -1;
+            const int t = base + (int)(threadIdx.x & 63);
+            bool want = t < end, w = false, f = false, s = false;
+            if (want) look(t, want, w, f, s);
+            todo = __ballot(want);
+            whole = __ballot(w);
+            full = __ballot(f);
+            skip = __ballot(s);
+        }
+        const int i = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        is_whole = whole >> i & 1;
+        is_full = full >> i & 1;
+        is_skip = skip >> i & 1;
+        return base + i;
+    }
+};
 
 constexpr int kCachedKeys = 32;            // keys of a wave's tile
 
@@ -267,7 +355,7 @@ template <typename T> int launch_attention_dkv(const AttnArgs &a, int dp, hipStr
 template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st);
 
 #define FLK_ATTN_LAUNCH(KERNEL, GRID)                                                                                        \
-    const bool mod = a.cap > 0.f || a.slopes != nullptr;                                                                     \
+    const bool mod = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);                                                                   \
     if (dp == 32) { if (mod) hipLaunchKernelGGL((KERNEL<T, 32, true>), GRID, dim3(kAttnThreads), 0, st, a);                  \
                     else hipLaunchKernelGGL((KERNEL<T, 32, false>), GRID, dim3(kAttnThreads), 0, st, a); }                   \
     else if (dp == 64) { if (mod) hipLaunchKernelGGL((KERNEL<T, 64, true>), GRID, dim3(kAttnThreads), 0, st, a);             \

@@ -1,11 +1,15 @@
 // Attention, forward: one pass over the keys with a running maximum and sum (gfx950).  Compiled once per element type.
 //
 // A workgroup owns 128 queries of one head, a wave 32 of them, with its queries and its 32 x d output in registers; tiles of
-// keys and values go through LDS.  The maximum is kept per row and the output rescaled only when some row of the wave found a
-// larger one.  Keys, values and probabilities never leave the chip.
+// keys and values go through LDS, the next one on its way while the present one is used.  The output is rescaled only when
+// some row of the wave found a maximum well above the one in use.  Scores and probabilities never leave the registers.
 #include "attention_common.h"
 
 namespace flk {
+
+// A maximum is taken over only when a row exceeds the present one by this much (in units of log 2): weights then lie below
+// 2^kSlack, which every type holds, and most tiles after the first need no rescaling.
+constexpr float kSlack = 6.f;
 
 template <typename T, int DP, bool MOD>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs p) {
@@ -13,8 +17,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
     constexpr int TK = AT::kTile, KB = TK / 32, C = DP / AT::KS, DB = DP / 32, ST = 32 / AT::KS;
-    __shared__ __align__(16) char lds_k[TK * TL::RB];
-    __shared__ __align__(16) char lds_v[TK * TL::RB];
+    typedef Feed<T, DP, TK> FD;
+    constexpr int kTileBytes = TK * TL::RB;
+    __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ int lds_doc[8];
     __shared__ int lds_bad;
 
@@ -27,15 +32,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
     const int off = p.sk - p.sq;
     const int i0 = tile_q * kAttnRows, row = i0 + wave * 32 + (lane & 31);
     const bool live = row < p.sq;
-    const int pos = row + off;
-    const int pos_lo = i0 + wave * 32 + off;                       // first position of this wave
+    const int pos = row + off, pos_lo = i0 + wave * 32 + off;
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;           // behind the last position of the workgroup
     const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
     const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;   // last key this row sees
 
     const T *qrow = (const T *)p.q + b * p.qs.b + h * p.qs.h + (int64_t)row * p.qs.s;
-    const T *kbase = (const T *)p.k + b * p.ks.b + hk * p.ks.h;
-    const T *vbase = (const T *)p.v + b * p.vs.b + hk * p.vs.h;
+    typename TL::Lane at_lane;
+    at_lane.init();
+    FD feed_k, feed_v;
+    feed_k.init((const T *)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, p.d, p.vec);
+    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec);
     frag qf[C];
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -45,123 +53,175 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
     }
 
     // documents: this row's id (no key has -2) and the span of the wave's and of the workgroup's rows
-    int dq = 0, w_lo = 0, w_hi = 0;
-    int2 wg_span = {0, 0};
-    const int *docs = p.docs != nullptr ? p.docs + b * p.docs_b : nullptr;
+    int id = 0;
+    int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
+    const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
     if (threadIdx.x == 0) lds_bad = -1;
-    if (docs != nullptr) {
-        const int raw = live ? max(docs[pos], -1) : -1;
-        w_lo = wave_min(raw);
-        w_hi = wave_max(raw);
-        if (lane == 0) { lds_doc[wave] = w_lo; lds_doc[4 + wave] = w_hi; }
-        dq = raw < 0 ? -2 : raw;
+    if (p.docs != nullptr) {
+        const int raw = live ? ids[pos] : -1;
+        span = {wave_min(raw), wave_max(raw)};
+        if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
+        id = raw < 0 ? -2 : raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
     }
-
     const int key_end = p.causal ? max(min(pos_end, p.sk), prefix) : p.sk;
-    const int tiles = key_end > 0 ? (key_end + TK - 1) / TK : 0;
+    TileWalk walk;
+    walk.start(0, key_end > 0 ? (key_end + TK - 1) / TK : 0);
+    const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
+        const int k0 = t * TK, k1 = k0 + TK;
+        const bool inside = k1 <= p.sk, in_prefix = !p.causal || k1 <= prefix;
+        whole = inside && (in_prefix || k1 - 1 <= i0 + off);
+        full = inside && (in_prefix || k1 - 1 <= pos_lo);
+        skip = p.causal && k0 > pos_lo + 31 && k0 >= prefix;
+        if (p.docs != nullptr) {
+            const int2 s = doc_span(ranges, k0, min(k1, p.sk));
+            want = docs_meet(s, wg_span);
+            whole = whole && docs_same(s, wg_span);
+            full = full && docs_same(s, span);
+            skip = skip || !docs_meet(s, span);
+        }
+    };
 
     fx16 o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) o[db] = fx16{};
-    float m = -kInf, l = 0.f;
+    float m = -kInf, l = 0.f;                                      // m in units of log 2
+    const float unit = p.scale * kScoreUnit;
 
-    for (int base = 0; base < tiles; base += 64) {
-        bool want = base + lane < tiles;
-        if (docs != nullptr && want) {
-            const int k0 = (base + lane) * TK;
-            want = docs_meet(doc_span(ranges, k0, min(k0 + TK, p.sk)), wg_span);
+    int buf = 0, tile = walk.next(look);
+    bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
+    if (tile >= 0) {
+        feed_k.issue(lds, tile * TK, min(TK, p.sk - tile * TK));
+        feed_v.issue(lds + kTileBytes, tile * TK, min(TK, p.sk - tile * TK));
+    }
+    while (tile >= 0) {
+        const int k0 = tile * TK;
+        const char *lds_k = lds + buf * 2 * kTileBytes, *lds_v = lds_k + kTileBytes;
+        const int next = walk.next(look);
+        FD::wait();
+        __syncthreads();                                           // this tile is there, the one before has been read
+        buf ^= 1;
+        if (next >= 0) {
+            feed_k.issue(lds + buf * 2 * kTileBytes, next * TK, min(TK, p.sk - next * TK));
+            feed_v.issue(lds + buf * 2 * kTileBytes + kTileBytes, next * TK, min(TK, p.sk - next * TK));
         }
-        for (uint64_t todo = __ballot(want); todo != 0; todo &= todo - 1) {
-            const int tile = base + __builtin_ctzll(todo), k0 = tile * TK, rows = min(TK, p.sk - k0);
-            // whether this tile needs no mask, for the workgroup (causal side: its first row) and for this wave
-            bool doc_full = true, wave_doc_full = true;
-            if (docs != nullptr) {
-                const int2 s = doc_span(ranges, k0, k0 + rows);
-                doc_full = s.x == s.y && s.x >= 0 && wg_span.x == s.x && wg_span.y == s.x;
-                wave_doc_full = s.x == s.y && s.x >= 0 && w_lo == s.x && w_hi == s.x;
-            }
-            const bool in_prefix = k0 + TK <= prefix;
-            const bool whole = rows == TK && doc_full && (!p.causal || in_prefix || k0 + TK - 1 <= i0 + off);
-            const bool full = rows == TK && wave_doc_full && (!p.causal || in_prefix || k0 + TK - 1 <= pos_lo);
-            Stage<T, DP, TK> sk, sv;
-            sk.load(kbase + (int64_t)k0 * p.ks.s, p.ks.s, rows, p.d, p.vec);
-            sv.load(vbase + (int64_t)k0 * p.vs.s, p.vs.s, rows, p.dv_d, p.vec);
-            __syncthreads();                                       // the previous tile has been read
-            sk.store(lds_k);
-            sv.store(lds_v);
-            if (!whole && sv.nonfinite()) lds_bad = tile;
+        bool careful = false;
+        if (!whole) {
+            if (FD::nonfinite(lds_v)) lds_bad = tile;
             __syncthreads();
-            const bool careful = !whole && lds_bad == tile;
-            // a wave none of whose rows sees anything here
-            if (p.causal && k0 > pos_lo + 31 && k0 >= prefix) continue;
-
-            fx16 s[KB];
-            float top = -kInf;
+            careful = lds_bad == tile;
+        }
+        fx16 s[KB];
+        if (!skip) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 s[kb] = fx16{};
 #pragma unroll
-                for (int c = 0; c < C; c++) s[kb] = AT::mma(TL::rows(lds_k, 32 * kb, c), qf[c], s[kb]);
+                for (int c = 0; c < C; c++) s[kb] = AT::mma(TL::rows(lds_k, at_lane, 32 * kb, c), qf[c], s[kb]);
             }
+            if constexpr (MOD) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        float t;
+                        s[kb][r] = score<T>(p, s[kb][r], slope, pos - (k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3)), t);
+                    }
+            }
+            if (!full) {
+                const int lim = last - k0 - 4 * half;
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[kb][r] = 32 * kb + 8 * (r >> 2) + (r & 3) <= lim ? s[kb][r] : -kInf;
+                if (p.docs != nullptr) {
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            const int4 t = *(const int4 *)(ids + min(k0 + 32 * kb, (p.doc_blocks - 1) * kDocBlock) + 8 * g + 4 * half);
+                            s[kb][4 * g] = t.x == id ? s[kb][4 * g] : -kInf;
+                            s[kb][4 * g + 1] = t.y == id ? s[kb][4 * g + 1] : -kInf;
+                            s[kb][4 * g + 2] = t.z == id ? s[kb][4 * g + 2] : -kInf;
+                            s[kb][4 * g + 3] = t.w == id ? s[kb][4 * g + 3] : -kInf;
+                        }
+                }
+            }
+            float top = -kInf;
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3);
-                    float t, x = score<T, MOD>(p, s[kb][r], slope, pos, key, t);
-                    if (!full) {
-                        bool see = key < p.sk && (!p.causal || key <= pos || key < prefix);
-                        if (docs != nullptr) see = see && docs[min(key, p.sk - 1)] == dq;
-                        x = see ? x : -kInf;
-                    }
-                    s[kb][r] = x;
-                    top = fmaxf(top, x);
-                }
+                for (int r = 0; r < 16; r++) top = fmaxf(top, s[kb][r]);
             top = fmaxf(top, other_half(top));
-            if (__any(top > m)) {
-                const float next = fmaxf(m, top);
-                const float a = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - next);
+            if constexpr (!MOD) top *= unit;
+            if (__any(top > m + (m == -kInf ? 0.f : kSlack))) {
+                const float next_m = fmaxf(m, top);
+                const float a = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - next_m);
                 l *= a;
-                m = next;
+                m = next_m;
 #pragma unroll
                 for (int db = 0; db < DB; db++) o[db] *= a;
             }
             const float base_m = m == -kInf ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};                   // short chains: long ones would cost float data digits
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r] - base_m);
-                    l += s[kb][r];
+                    s[kb][r] = __builtin_amdgcn_exp2f(MOD ? s[kb][r] - base_m : __builtin_fmaf(s[kb][r], unit, -base_m));
+                    sum[r & 3] += s[kb][r];
                 }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        if (careful) {
+            if (!skip) {                                           // through copies, so that s and o stay in registers elsewhere
+                fx16 w[KB], x[DB];
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) w[kb] = s[kb];
+#pragma unroll
+                for (int db = 0; db < DB; db++) x[db] = o[db];
+                spread_nonfinite<T, DP, KB, DB>(lds_v, w, x);
+#pragma unroll
+                for (int db = 0; db < DB; db++) o[db] = x[db];
+            }
+            __syncthreads();
+            FD::clean_share(lds + (buf ^ 1) * 2 * kTileBytes + kTileBytes);
+            __syncthreads();
+        }
+        if (!skip) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int st = 0; st < ST; st++) {
                     const frag pf = pack<T>(s[kb], st);
 #pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        const frag vf = TL::cols(lds_v, 32 * kb + AT::KS * st, 32 * db);
-                        if (careful) o[db] = mma_careful<T>(vf, pf, o[db]);
-                        else o[db] = AT::mma(vf, pf, o[db]);
-                    }
+                    for (int db = 0; db < DB; db++) o[db] = AT::mma(TL::cols(lds_v, at_lane, 32 * kb + AT::KS * st, db), pf, o[db]);
                 }
         }
+        tile = next;
+        whole = walk.is_whole;
+        full = walk.is_full;
+        skip = walk.is_skip;
     }
     l += other_half(l);
     if (!live) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;                    // a row that sees nothing is zero
-    T *orow = (T *)p.o + (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
+    const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
+    T *orow = (T *)p.o + at, *rest = p.rest != nullptr ? (T *)p.rest + at : nullptr;
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (c < p.dv_d) orow[c] = (T)(o[db][r] * inv);
+            if (c < p.dv_d) {
+                const float x = o[db][r] * inv;
+                const T y = (T)x;
+                orow[c] = y;
+                if (rest != nullptr) rest[c] = (T)(x - (float)y);
+            }
         }
     if (half == 0 && p.lse != nullptr)
         p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : m * kLn2 + __logf(l);

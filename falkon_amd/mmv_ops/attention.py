@@ -98,27 +98,29 @@ def _workspace(nbytes: int, dev) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _forward(q, k, v, slopes, scale, softcap, causal, prefix, documents, want_lse):
+def _forward(q, k, v, slopes, scale, softcap, causal, prefix, documents, want_lse, train=False):
     lib = _backend.load()
     b, sq, hq, d = q.shape
     sk, hk, dv = k.shape[1], k.shape[2], v.shape[3]
     out = torch.empty((b, sq, hq, dv), dtype=q.dtype, device=q.device)
+    # what rounding takes from 16-bit results: dout.out, which the backward pass subtracts from every term, needs it
+    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     lse = torch.empty((b, hq, sq), dtype=torch.float32, device=q.device) if want_lse else None
     nbytes = lib.flk_attention_workspace_bytes(b, sk, 1) if documents is not None else 0
     ws = _workspace(nbytes, q.device)
     with _current(q.device):
         rc = lib.flk_attention(*_bsh(q), *_bsh(k), *_bsh(v), b, sq, sk, hq, hk, d, dv, scale, softcap, _ptr(slopes), causal,
                                _ptr(prefix), _ptr(documents), documents.stride(0) if documents is not None else 0,
-                               out.data_ptr(), _ptr(lse), _DTYPE_CODE[q.dtype], _ptr(ws), nbytes, _stream_handle(q.device))
+                               out.data_ptr(), _ptr(rest), _ptr(lse), _DTYPE_CODE[q.dtype], _ptr(ws), nbytes, _stream_handle(q.device))
     _backend.raise_for_status(rc, "flk_attention")
-    return out, lse
+    return out, rest, lse
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, scale, softcap, causal, prefix, documents):
-        out, lse = _forward(q, k, v, slopes, scale, softcap, causal, prefix, documents, True)
-        ctx.save_for_backward(q, k, v, slopes, prefix, documents, out, lse)
+        out, rest, lse = _forward(q, k, v, slopes, scale, softcap, causal, prefix, documents, True, True)
+        ctx.save_for_backward(q, k, v, slopes, prefix, documents, out, rest, lse)
         ctx.plain = scale, softcap, causal
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -126,7 +128,7 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, slopes, prefix, documents, out, lse = ctx.saved_tensors
+        q, k, v, slopes, prefix, documents, out, rest, lse = ctx.saved_tensors
         scale, softcap, causal = ctx.plain
         need_q, need_k, need_v, need_slopes = ctx.needs_input_grad[:4]
         lib = _backend.load()
@@ -144,7 +146,7 @@ class _AttentionFn(torch.autograd.Function):
         ws = _workspace(nbytes, dev)
         with _current(dev):
             rc = lib.flk_attention_backward(
-                *_bsh(q), *_bsh(k), *_bsh(v), out.data_ptr(), lse.data_ptr(), *_bsh(dout), b, sq, sk, hq, hk, d, dv, scale, softcap,
+                *_bsh(q), *_bsh(k), *_bsh(v), out.data_ptr(), _ptr(rest), lse.data_ptr(), *_bsh(dout), b, sq, sk, hq, hk, d, dv, scale, softcap,
                 _ptr(slopes), causal, _ptr(prefix), _ptr(documents), documents.stride(0) if documents is not None else 0,
                 _ptr(dq), _ptr(dk), _ptr(dv_), _ptr(dslopes), _DTYPE_CODE[q.dtype], _ptr(ws), nbytes, _stream_handle(dev))
         _backend.raise_for_status(rc, "flk_attention_backward")
@@ -204,7 +206,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (slopes is not None and slopes.requires_grad)):
         out, lse = _AttentionFn.apply(q, k, v, slopes, scale, softcap, bool(causal), prefix, documents)
     else:
-        out, lse = _forward(q, k, v, slopes, scale, softcap, bool(causal), prefix, documents, return_lse)
+        out, _, lse = _forward(q, k, v, slopes, scale, softcap, bool(causal), prefix, documents, return_lse)
     if matrix:
         out, lse = out[0, :, 0], lse[0, 0] if return_lse else None
     return (out, lse) if return_lse else out

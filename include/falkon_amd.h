@@ -320,8 +320,9 @@ int flk_layer_norm_backward(const void *x, int64_t rows, int64_t d, int64_t x_rs
  * causal: keys behind pos_i are hidden, except the first prefix[b] of them (prefix: b ints or NULL, causal only).
  * documents: b x sk ints (rows documents_b apart) or NULL: a row sees keys of its own number only, and nothing if that
  * is negative; needs sq <= sk.  out: b x sq x hq x dv, contiguous.  lse: b x hq x sq floats (the logarithm of the row's sum,
- * -inf for a row that sees nothing), or NULL where no backward pass follows.
- * flk_attention_backward: from out, lse and dout the gradients dq, dk, dv (contiguous, like q, k, v; dk and dv both or
+ * -inf for a row that sees nothing), or NULL where no backward pass follows.  rest: like out, or NULL: what rounding to 16
+ * bits took from out, which the backward pass adds again (not used for FLK_F32).
+ * flk_attention_backward: from out, rest (or NULL), lse and dout the gradients dq, dk, dv (contiguous, like q, k, v; dk and dv both or
  * neither) and dslopes (hq floats); each may be NULL.  Sums are made in a fixed order: the same run to run. */
 int64_t flk_attention_max_d(int dtype);
 
@@ -331,14 +332,14 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
                   const void *v, int64_t v_b, int64_t v_s, int64_t v_h,
                   int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
                   double scale, double softcap, const float *slopes, int causal, const int *prefix,
-                  const int *documents, int64_t documents_b, void *out, float *lse, int dtype,
+                  const int *documents, int64_t documents_b, void *out, void *rest, float *lse, int dtype,
                   void *workspace, size_t workspace_bytes, void *stream);
 
 size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
                                               int with_dslopes, int with_documents);
 
 int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
-                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const float *lse,
+                           const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const void *rest, const float *lse,
                            const void *dout, int64_t do_b, int64_t do_s, int64_t do_h,
                            int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
                            double scale, double softcap, const float *slopes, int causal, const int *prefix,

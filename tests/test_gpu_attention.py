@@ -186,7 +186,10 @@ def test_extreme_scores(dtype):
     k[:, 170] = q[:, 50, :, :] * 8
     _check(q * 4, k, v, do, scale=1.0)
     out = attention(q, torch.ones_like(k) * 50, torch.ones_like(v))
-    assert bool((out == 1).all())
+    # 300 equal weights p: out is the sum of p * 1 over the sum of p, two float summations of the same numbers, each within
+    # 300 * 2^-24 of the true sum whatever their order, and one division; for 16-bit types that rounds to 1 (half a step
+    # is 2^-11 or more) and p, within 2^-15 of a power of two times 1, adds nothing to it
+    assert float((out.double() - 1).abs().max()) <= (601 * 2.0 ** -24 if dtype == torch.float32 else 0.0)
 
 
 @pytest.mark.gpu
@@ -436,8 +439,8 @@ def test_c_entry_refusals():
     from falkon_amd import _backend
     lib = _backend.load()
     one = 16                                                # any address: never read
-    names = "q qb qs qh k kb ks kh v vb vs vh b sq sk hq hk d dv scale cap slopes causal prefix docs docs_b out lse dt ws wsb st".split()
-    base = dict(zip(names, [one, 8, 8, 8] * 3 + [1, 5, 7, 4, 2, 8, 8, 1.0, 0.0, None, 0, None, None, 0, one, None, 0, None, 0, None]))
+    names = "q qb qs qh k kb ks kh v vb vs vh b sq sk hq hk d dv scale cap slopes causal prefix docs docs_b out rest lse dt ws wsb st".split()
+    base = dict(zip(names, [one, 8, 8, 8] * 3 + [1, 5, 7, 4, 2, 8, 8, 1.0, 0.0, None, 0, None, None, 0, one, None, None, 0, None, 0, None]))
     call = lambda **kw: lib.flk_attention(*[{**base, **kw}[n] for n in names])  # noqa: E731
     assert call(b=0) == 0 and call(sq=0) == 0
     for bad in (dict(b=-1), dict(hq=0), dict(hq=3), dict(d=0), dict(dt=1), dict(dt=2), dict(cap=-1.0), dict(cap=math.nan), dict(prefix=one),
@@ -448,7 +451,7 @@ def test_c_entry_refusals():
     need = lib.flk_attention_workspace_bytes(1, 7, 1)
     assert need > 0 and lib.flk_attention_workspace_bytes(1, 7, 0) == 0
     assert call(docs=one, ws=one, wsb=need - 1) == _backend.FLK_ENOMEM and call(docs=one, wsb=need) == _backend.FLK_ENOMEM
-    bnames = ("q qb qs qh k kb ks kh v vb vs vh out lse do dob dos doh b sq sk hq hk d dv scale cap slopes causal prefix docs docs_b "
+    bnames = ("q qb qs qh k kb ks kh v vb vs vh out rest lse do dob dos doh b sq sk hq hk d dv scale cap slopes causal prefix docs docs_b "
               "dq dk dvo dsl dt ws wsb st").split()
     bbase = {**base, "lse": one, "do": one, "dob": 8, "dos": 8, "doh": 8, "dq": one, "dk": one, "dvo": one, "dsl": None}
     back = lambda **kw: lib.flk_attention_backward(*[{**bbase, **kw}[n] for n in bnames])  # noqa: E731
