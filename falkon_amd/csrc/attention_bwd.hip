@@ -12,7 +12,7 @@
 
 namespace flk {
 
-template <typename T, int DP, bool MOD>
+template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_dq_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const bool live = row < p.sq;
     const int pos = row + off, pos_lo = i0 + wave * 32 + off;
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;
-    const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
+    const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
     const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
     const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;
 
@@ -109,7 +109,6 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     for (int db = 0; db < DB; db++) acc[db] = fx16{};
     // sum_j dS |dist|, sum_j dS and sum_j P |dist|: the second is what the rounding of out left in delta, and is taken out
     float far = 0.f, left = 0.f, reach = 0.f;
-    const float unit = p.scale * kScoreUnit;
 
     int buf = 0, tile = walk.next(look);
     bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
@@ -134,6 +133,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         }
         if (!skip) {
             const int lim = last - k0 - 4 * half;
+            const float at_key = (float)(pos - k0 - 4 * half);
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 fx16 s = {}, dp = {};
@@ -159,24 +159,21 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                 }
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    float e, g, t = 0.f;
-                    if constexpr (MOD) {
-                        const int dist = pos - (k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3));
-                        e = __builtin_amdgcn_exp2f(score<T>(p, s[r], slope, dist, t) - lse);
-                        g = e * (dp[r] - delta);
-                        if (!full) { e = hide[r] ? 0.f : e; g = hide[r] ? 0.f : g; }
+                    float e, g, grad = 1.f;
+                    const float dist = at_key - (float)(32 * kb + 8 * (r >> 2) + (r & 3));
+                    if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse));
+                    else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse);
+                    g = e * (dp[r] - delta);
+                    if (!full) g = hide[r] ? 0.f : g;
+                    if constexpr ((MOD & kDecay) != 0) {
                         if (p.dslopes_part != nullptr) {
-                            const float a = __builtin_fabsf((float)dist);
-                            far += g * a;
+                            if (!full) e = hide[r] ? 0.f : e;
+                            far += g * __builtin_fabsf(dist);
                             left += g;
-                            reach += e * a;
+                            reach += e * __builtin_fabsf(dist);
                         }
-                        if (p.cap > 0.f) g *= 1.f - t * t;
-                    } else {
-                        e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit, -lse));
-                        g = e * (dp[r] - delta);
-                        if (!full) g = hide[r] ? 0.f : g;
                     }
+                    if constexpr ((MOD & kCap) != 0) g *= grad;
                     s[r] = g;
                 }
 #pragma unroll
@@ -192,7 +189,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         full = walk.is_full;
         skip = walk.is_skip;
     }
-    if (MOD && p.dslopes_part != nullptr) {                        // in a fixed order: lanes, then waves
+    if ((MOD & kDecay) != 0 && p.dslopes_part != nullptr) {                        // in a fixed order: lanes, then waves
         far += other_half(far);
         left += other_half(left);
         reach += other_half(reach);
@@ -211,11 +208,11 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (c < p.d) out[c] = (T)(acc[db][r] * p.scale);
+            if (c < p.d) out[c] = (T)(acc[db][r] * (p.scale * score.kGrad));
         }
 }
 
-template <typename T, int DP, bool MOD>
+template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
@@ -284,12 +281,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
     fx16 dk[DB], dv[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
-    const float unit = p.scale * kScoreUnit;
 
     const int h_lo = p.group * split / p.splits, h_hi = p.group * (split + 1) / p.splits;
     for (int hg = h_lo; hg < h_hi; hg++) {
         const int h = hk * p.group + hg;
-        const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
+        const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
         const float *stats = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad;
         FD feed_q, feed_g;
         feed_q.init((const T *)p.q + b * p.qs.b + h * p.qs.h, p.qs.s, p.d, p.vec);
@@ -334,6 +330,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
             }
             if (!skip) {
                 const int lim = first - i0 - 4 * half;
+                const float at_row = (float)(i0 + off + 4 * half - key);
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++) {
                     fx16 s = {}, dp = {};
@@ -361,11 +358,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int r = 4 * g4 + i;
-                            float e, g, t = 0.f;
-                            if constexpr (MOD) e = __builtin_amdgcn_exp2f(score<T>(p, s[r], slope, i0 + a + i + off - key, t) - lse[i]);
-                            else e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit, -lse[i]));
+                            float e, g, grad = 1.f;
+                            if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse[i]));
+                            else e = __builtin_amdgcn_exp2f(score(s[r], at_row + (float)(32 * qb + 8 * g4 + i), grad) - lse[i]);
                             g = e * (dp[r] - delta[i]);
-                            if (MOD && p.cap > 0.f) g *= 1.f - t * t;
+                            if constexpr ((MOD & kCap) != 0) g *= grad;
                             if (!whole) e = __builtin_fmaf(delta[i], 0.f, e);
                             if (!full) { e = hide[i] ? 0.f : e; g = hide[i] ? 0.f : g; }
                             s[r] = e;
@@ -399,7 +396,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (c < p.d) ok[c] = (T)(dk[db][r] * p.scale);
+                if (c < p.d) ok[c] = (T)(dk[db][r] * (p.scale * Score<T, MOD>::kGrad));
                 if (c < p.dv_d) ov[c] = (T)dv[db][r];
             }
     } else {                                                       // parts in float, added by attention_join_kernel
@@ -410,7 +407,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (c < p.d) ok[c] = dk[db][r] * p.scale;
+                if (c < p.d) ok[c] = dk[db][r] * (p.scale * Score<T, MOD>::kGrad);
                 if (c < p.dv_d) ov[c] = dv[db][r];
             }
     }
@@ -419,10 +416,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
 template <typename T> int launch_attention_dq(const AttnArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows)));
     FLK_ATTN_LAUNCH(attention_dq_kernel, grid)
+    return FLK_OK;
 }
 template <typename T> int launch_attention_dkv(const AttnArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.splits * ((a.sk + kAttnRows - 1) / kAttnRows)));
     FLK_ATTN_LAUNCH(attention_dkv_kernel, grid)
+    return FLK_OK;
 }
 template int launch_attention_dq<attn_t>(const AttnArgs &, int, hipStream_t);
 template int launch_attention_dkv<attn_t>(const AttnArgs &, int, hipStream_t);

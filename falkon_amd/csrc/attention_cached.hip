@@ -9,7 +9,7 @@
 
 namespace flk {
 
-template <typename T, int DP, bool MOD>
+template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_cached_kernel(CachedArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const bool live = r < n_rows;
     const int t = r / p.group, h = hk * p.group + r % p.group;
     const int pos = len - p.t + t, pos_lo = len - p.t + rb * 32 / p.group;
-    const float slope = MOD && p.slopes != nullptr && live ? p.slopes[h] : 0.f;
+    const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr && live ? p.slopes[h] : 0.f);
     // this workgroup's keys, in whole tiles
     const int all = (len + TK - 1) / TK, per = (all + p.splits - 1) / p.splits;
     const int tile_lo = min(split * per, all), tile_hi = min(tile_lo + per, all);
@@ -87,13 +87,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int key = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
-            float th, x;
-            if constexpr (!MOD) x = s[i] * (p.scale * kScoreUnit);
-            else {
-                x = s[i] * p.scale;
-                if (p.cap > 0.f) { th = tanh_of<T>(x * __builtin_amdgcn_rcpf(p.cap)); x = p.cap * th; }
-                x = (x - slope * __builtin_fabsf((float)(pos - key))) * kScoreUnit;
-            }
+            float grad, x = score(s[i], (float)(pos - key), grad);
             if (!full) x = key <= pos ? x : -kInf;                 // pos < len: nothing behind the sequence either
             s[i] = x;
             top = fmaxf(top, x);
@@ -193,13 +187,9 @@ __global__ void __launch_bounds__(kAttnThreads) attention_cached_join_kernel(Cac
     ((T *)p.out)[i] = (T)(sum == 0.f ? 0.f : x / sum);
 }
 
-#define FLK_CACHED(DP)                                                                                                           \
-    if (a.cap > 0.f || a.slopes != nullptr) hipLaunchKernelGGL((attention_cached_kernel<T, DP, true>), grid, dim3(kAttnThreads), 0, st, a); \
-    else hipLaunchKernelGGL((attention_cached_kernel<T, DP, false>), grid, dim3(kAttnThreads), 0, st, a);
 template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.blocks_r * a.splits));
-    if (dp == 32) { FLK_CACHED(32) } else if (dp == 64) { FLK_CACHED(64) } else if (dp == 96) { FLK_CACHED(96) } else { FLK_CACHED(128) }
-    FLK_LAUNCH_CHECK("attention_cached_kernel");
+    FLK_ATTN_LAUNCH(attention_cached_kernel, grid)
     if (a.splits > 1) {
         const int64_t n = (int64_t)a.b * a.t * a.hq * a.dv_d;
         hipLaunchKernelGGL((attention_cached_join_kernel<T>), dim3((unsigned)((n + kAttnThreads - 1) / kAttnThreads)), dim3(kAttnThreads), 0, st, a);

@@ -267,23 +267,45 @@ template <typename T, int DP, int TR> struct Feed {
     }
 };
 
-// tanh through one exponential; near zero, where 1 - 2 / (1 + e) would cancel, the odd series (next term below 2^-25 at 1/4)
-template <typename T> __device__ __forceinline__ float tanh_of(float u) {
-    const float e = __builtin_amdgcn_exp2f(2.f * kScoreUnit * u);
-    const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e);
-    if constexpr (sizeof(T) == 2) return t;
-    const float w = u * u;
-    const float s = u * (1.f + w * (-1.f / 3 + w * (2.f / 15 + w * (-17.f / 315 + w * (62.f / 2835)))));
-    return __builtin_fabsf(u) < 0.25f ? s : t;
-}
+// What happens to the scores before the softmax.  A scale that is not positive goes with kDecay, whose rows look for their
+// maximum among the finished scores.
+constexpr int kPlain = 0, kCap = 1, kDecay = 2, kCapDecay = 3;
 
-// One score in units of log 2, and the tanh (for its derivative)
-template <typename T>
-__device__ __forceinline__ float score(const AttnArgs &p, float s, float slope, int dist, float &t) {
-    float x = s * p.scale;
-    if (p.cap > 0.f) { t = tanh_of<T>(x * __builtin_amdgcn_rcpf(p.cap)); x = p.cap * t; }
-    return (x - slope * __builtin_fabsf((float)dist)) * kScoreUnit;
-}
+// Scores x in units of log 2, and the derivative of the cap.  With r = 1 / (1 + exp(2 u)), u = scale s / cap:
+// cap tanh u = cap - 2 cap r, and its derivative in u is 4 cap r (1 - r).  Two transcendental instructions a score; r comes with an
+// error of 2^-24, so a score with one of cap 2^-22, far below what rounding the weights to 16 bits costs.  Float data take the odd
+// series instead where tanh is small and 1 - 2 r would cancel (its next term is below 2^-25 of the sum at u = 1/4).
+template <typename T, int MOD> struct Score {
+    static constexpr bool kHasCap = (MOD & 1) != 0, kHasDecay = (MOD & 2) != 0, kWide = sizeof(T) == 4;
+    float unit, in, out, slope;
+    __device__ __forceinline__ Score(float scale, float cap, float slope_) {
+        unit = scale * kScoreUnit;
+        in = kHasCap ? (kWide ? scale / cap : 2.f * kScoreUnit * scale / cap) : 0.f;
+        out = cap * kScoreUnit;
+        slope = slope_ * kScoreUnit;
+    }
+    __device__ __forceinline__ float r(float s) const { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * in)); }
+    // x of an inner product s at distance `dist`; `grad` gets the derivative by scale * s, a quarter of it for 16-bit data
+    __device__ __forceinline__ float operator()(float s, float dist, float &grad) const {
+        float x;
+        if constexpr (!kHasCap) x = s * unit;
+        else if constexpr (!kWide) {
+            const float a = r(s);
+            x = __builtin_fmaf(a, -2.f * out, out);
+            grad = __builtin_fmaf(-a, a, a);
+        } else {
+            const float u = s * in, w = u * u;
+            const float e = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kScoreUnit * u));
+            const float near = u * (1.f + w * (-1.f / 3 + w * (2.f / 15 + w * (-17.f / 315 + w * (62.f / 2835)))));
+            const float t = __builtin_fabsf(u) < 0.25f ? near : 1.f - 2.f * e;
+            x = t * out;
+            grad = 1.f - t * t;
+        }
+        if constexpr (kHasDecay) x = __builtin_fmaf(-slope, __builtin_fabsf(dist), x);
+        return x;
+    }
+    static constexpr float kGrad = kHasCap && !kWide ? 4.f : 1.f;   // what `grad` leaves to the end
+};
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 __device__ __forceinline__ int wave_min(int x) {
@@ -354,18 +376,23 @@ template <typename T> int launch_attention_dq(const AttnArgs &a, int dp, hipStre
 template <typename T> int launch_attention_dkv(const AttnArgs &a, int dp, hipStream_t st);
 template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st);
 
-#define FLK_ATTN_LAUNCH(KERNEL, GRID)                                                                                        \
-    const bool mod = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);                                                                   \
-    if (dp == 32) { if (mod) hipLaunchKernelGGL((KERNEL<T, 32, true>), GRID, dim3(kAttnThreads), 0, st, a);                  \
-                    else hipLaunchKernelGGL((KERNEL<T, 32, false>), GRID, dim3(kAttnThreads), 0, st, a); }                   \
-    else if (dp == 64) { if (mod) hipLaunchKernelGGL((KERNEL<T, 64, true>), GRID, dim3(kAttnThreads), 0, st, a);             \
-                         else hipLaunchKernelGGL((KERNEL<T, 64, false>), GRID, dim3(kAttnThreads), 0, st, a); }              \
-    else if (dp == 96) { if (mod) hipLaunchKernelGGL((KERNEL<T, 96, true>), GRID, dim3(kAttnThreads), 0, st, a);             \
-                         else hipLaunchKernelGGL((KERNEL<T, 96, false>), GRID, dim3(kAttnThreads), 0, st, a); }              \
-    else { if (mod) hipLaunchKernelGGL((KERNEL<T, 128, true>), GRID, dim3(kAttnThreads), 0, st, a);                          \
-           else hipLaunchKernelGGL((KERNEL<T, 128, false>), GRID, dim3(kAttnThreads), 0, st, a); }                           \
-    FLK_LAUNCH_CHECK(#KERNEL);                                                                                               \
-    return FLK_OK;
+inline int score_kind(float scale, float cap, const float *slopes) {
+    return (cap > 0.f ? kCap : kPlain) | (slopes != nullptr || !(scale > 0.f) ? kDecay : 0);
+}
+#define FLK_ATTN_KIND(KERNEL, DP, GRID)                                                                            \
+    {                                                                                                              \
+        if (kind == kPlain) hipLaunchKernelGGL((KERNEL<T, DP, kPlain>), GRID, dim3(kAttnThreads), 0, st, a);       \
+        else if (kind == kCap) hipLaunchKernelGGL((KERNEL<T, DP, kCap>), GRID, dim3(kAttnThreads), 0, st, a);      \
+        else if (kind == kDecay) hipLaunchKernelGGL((KERNEL<T, DP, kDecay>), GRID, dim3(kAttnThreads), 0, st, a);  \
+        else hipLaunchKernelGGL((KERNEL<T, DP, kCapDecay>), GRID, dim3(kAttnThreads), 0, st, a);                   \
+    }
+#define FLK_ATTN_LAUNCH(KERNEL, GRID)                              \
+    const int kind = score_kind(a.scale, a.cap, a.slopes);         \
+    if (dp == 32) FLK_ATTN_KIND(KERNEL, 32, GRID)                  \
+    else if (dp == 64) FLK_ATTN_KIND(KERNEL, 64, GRID)             \
+    else if (dp == 96) FLK_ATTN_KIND(KERNEL, 96, GRID)             \
+    else FLK_ATTN_KIND(KERNEL, 128, GRID)                          \
+    FLK_LAUNCH_CHECK(#KERNEL);
 
 #if defined(FLK_KF)
 #if FLK_KF == 0

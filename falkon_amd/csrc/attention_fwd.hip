@@ -11,7 +11,7 @@ namespace flk {
 // 2^kSlack, which every type holds, and most tiles after the first need no rescaling.
 constexpr float kSlack = 6.f;
 
-template <typename T, int DP, bool MOD>
+template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
@@ -34,7 +34,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
     const bool live = row < p.sq;
     const int pos = row + off, pos_lo = i0 + wave * 32 + off;
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;           // behind the last position of the workgroup
-    const float slope = MOD && p.slopes != nullptr ? p.slopes[h] : 0.f;
+    const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
+    constexpr bool kLate = MOD == kPlain || (MOD == kCap && sizeof(T) == 2);   // rising in s: the maximum is looked for before
     const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
     const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;   // last key this row sees
 
@@ -89,7 +90,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
 #pragma unroll
     for (int db = 0; db < DB; db++) o[db] = fx16{};
     float m = -kInf, l = 0.f;                                      // m in units of log 2
-    const float unit = p.scale * kScoreUnit;
 
     int buf = 0, tile = walk.next(look);
     bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
@@ -122,13 +122,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
 #pragma unroll
                 for (int c = 0; c < C; c++) s[kb] = AT::mma(TL::rows(lds_k, at_lane, 32 * kb, c), qf[c], s[kb]);
             }
-            if constexpr (MOD) {
+            if constexpr (!kLate) {
+                const float at = (float)(pos - k0 - 4 * half);
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        float t;
-                        s[kb][r] = score<T>(p, s[kb][r], slope, pos - (k0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3)), t);
+                        float grad;
+                        s[kb][r] = score(s[kb][r], at - (float)(32 * kb + 8 * (r >> 2) + (r & 3)), grad);
                     }
             }
             if (!full) {
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
 #pragma unroll
                 for (int r = 0; r < 16; r++) top = fmaxf(top, s[kb][r]);
             top = fmaxf(top, other_half(top));
-            if constexpr (!MOD) top *= unit;
+            if constexpr (kLate) { float grad; top = score(top, 0.f, grad); }
             if (__any(top > m + (m == -kInf ? 0.f : kSlack))) {
                 const float next_m = fmaxf(m, top);
                 const float a = m == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - next_m);
@@ -171,7 +172,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[kb][r] = __builtin_amdgcn_exp2f(MOD ? s[kb][r] - base_m : __builtin_fmaf(s[kb][r], unit, -base_m));
+                    if constexpr (MOD == kPlain) s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], score.unit, -base_m));
+                    else if constexpr (!kLate) s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r] - base_m);
+                    else {
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score.r(s[kb][r]), -2.f * score.out, score.out - base_m));
+                        s[kb][r] = full || s[kb][r] != -kInf ? e : 0.f;
+                    }
                     sum[r & 3] += s[kb][r];
                 }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
 template <typename T> int launch_attention_fwd(const AttnArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows)));
     FLK_ATTN_LAUNCH(attention_fwd_kernel, grid)
+    return FLK_OK;
 }
 template int launch_attention_fwd<attn_t>(const AttnArgs &, int, hipStream_t);
 
