@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         const int raw = live ? ids[pos] : -1;
         span = {wave_min(raw), wave_max(raw)};
         if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
-        id = raw < 0 ? -2 : raw;
+        id = raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
@@ -110,53 +110,65 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     // sum_j dS |dist|, sum_j dS and sum_j P |dist|: the second is what the rounding of out left in delta, and is taken out
     float far = 0.f, left = 0.f, reach = 0.f;
 
+    int place_id = -1, next_id = -1;                               // id of key k0 + lane, one tile ahead
+    const auto id_at = [&](int t) {
+        const int k = t * TK + lane;
+        return lane < TK && k < p.sk ? ids[k] : -1;
+    };
     int buf = 0, tile = walk.next(look);
     bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
     if (tile >= 0) {
         feed_k.issue(lds, tile * TK, min(TK, p.sk - tile * TK));
         feed_v.issue(lds + kTileBytes, tile * TK, min(TK, p.sk - tile * TK));
+        if (p.docs != nullptr) next_id = id_at(tile);
     }
     while (tile >= 0) {
         const int k0 = tile * TK;
         char *lds_k = lds + buf * 2 * kTileBytes, *lds_v = lds_k + kTileBytes;
         const int next = walk.next(look);
         FD::wait();
+        place_id = next_id;
         __syncthreads();
         buf ^= 1;
         if (next >= 0) {
             feed_k.issue(lds + buf * 2 * kTileBytes, next * TK, min(TK, p.sk - next * TK));
             feed_v.issue(lds + buf * 2 * kTileBytes + kTileBytes, next * TK, min(TK, p.sk - next * TK));
+            if (p.docs != nullptr) next_id = id_at(next);
         }
         if (!whole) {                                              // a row that sees what this removes has a lse of NaN
             FD::clean_share(lds_k);
             __syncthreads();
         }
         if (!skip) {
-            const int lim = last - k0 - 4 * half;
+            Seen seen;
+            if (!full) {
+                uint64_t see = low_bits(last + 1 - k0);
+                if (p.docs != nullptr) see &= same_id(place_id, id);
+                seen = seen_from(see);
+            }
             const float at_key = (float)(pos - k0 - 4 * half);
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 fx16 s = {}, dp = {};
+                {   // fragments of keys and values, read up to four steps ahead of their products
+                    constexpr int W = C < 4 ? C : 4;
+                    frag kf[W], vf[W];
 #pragma unroll
-                for (int c = 0; c < C; c++) {
-                    s = AT::mma(TL::rows(lds_k, at_lane, 32 * kb, c), qf[c], s);
-                    dp = AT::mma(TL::rows(lds_v, at_lane, 32 * kb, c), gf[c], dp);
-                }
-                bool hide[16];
-                if (!full) {
+                    for (int i = 0; i < W; i++) { kf[i] = TL::rows(lds_k, at_lane, 32 * kb, i); vf[i] = TL::rows(lds_v, at_lane, 32 * kb, i); }
+                    FLK_KEEP_ORDER();
 #pragma unroll
-                    for (int r = 0; r < 16; r++) hide[r] = 32 * kb + 8 * (r >> 2) + (r & 3) > lim;
-                    if (p.docs != nullptr) {
-#pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            const int4 t = *(const int4 *)(ids + min(k0 + 32 * kb, (p.doc_blocks - 1) * kDocBlock) + 8 * g + 4 * half);
-                            hide[4 * g] |= t.x != id;
-                            hide[4 * g + 1] |= t.y != id;
-                            hide[4 * g + 2] |= t.z != id;
-                            hide[4 * g + 3] |= t.w != id;
-                        }
+                    for (int c = 0; c < C; c++) {
+                        s = AT::mma(kf[c % W], qf[c], s);
+                        dp = AT::mma(vf[c % W], gf[c], dp);
+                        if (c + W < C) { kf[c % W] = TL::rows(lds_k, at_lane, 32 * kb, c + W); vf[c % W] = TL::rows(lds_v, at_lane, 32 * kb, c + W); }
+                        FLK_KEEP_ORDER();
                     }
                 }
+                constexpr int F = ST * DB;
+                frag kt[F];
+#pragma unroll
+                for (int i = 0; i < F; i++) kt[i] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * (i / DB), i % DB);
+                FLK_KEEP_ORDER();
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     float e, g, grad = 1.f;
@@ -164,10 +176,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                     if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse));
                     else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse);
                     g = e * (dp[r] - delta);
-                    if (!full) g = hide[r] ? 0.f : g;
+                    if (!full) g = seen.or_zero(g, kb, r);
                     if constexpr ((MOD & kDecay) != 0) {
                         if (p.dslopes_part != nullptr) {
-                            if (!full) e = hide[r] ? 0.f : e;
+                            if (!full) e = seen.or_zero(e, kb, r);
                             far += g * __builtin_fabsf(dist);
                             left += g;
                             reach += e * __builtin_fabsf(dist);
@@ -178,9 +190,9 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                 }
 #pragma unroll
                 for (int st = 0; st < ST; st++) {
-                    const frag gfr = pack<T>(s, st);
+                    const frag ds = pack<T>(s, st);
 #pragma unroll
-                    for (int db = 0; db < DB; db++) acc[db] = AT::mma(TL::cols(lds_k, at_lane, 32 * kb + AT::KS * st, db), gfr, acc[db]);
+                    for (int db = 0; db < DB; db++) acc[db] = AT::mma(kt[st * DB + db], ds, acc[db]);
                 }
             }
         }
@@ -222,7 +234,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
     constexpr int kTileBytes = TQ * TL::RB;
     __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ __align__(16) float lds_stat[2][2][TQ];             // lse and delta of a tile's rows
-    __shared__ __align__(16) int lds_id[2][TQ];
     __shared__ int lds_doc[8];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -256,7 +267,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
         const int raw = live ? ids[key] : -1;
         span = {wave_min(raw), wave_max(raw)};
         if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
-        id = raw < 0 ? -2 : raw;
+        id = raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
@@ -290,9 +301,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
         FD feed_q, feed_g;
         feed_q.init((const T *)p.q + b * p.qs.b + h * p.qs.h, p.qs.s, p.d, p.vec);
         feed_g.init((const T *)p.dout + b * p.dos.b + h * p.dos.h, p.dos.s, p.dv_d, p.vec);
-        // a tile's statistics (padded to whole tiles of 128 rows) and ids pass through registers of its first threads
+        // a tile's statistics (padded to whole tiles of 128 rows) pass through registers of its first threads
         float r_lse = 0.f, r_delta = 0.f;
-        int r_id = -1;
+        int place_id = -1, next_id = -1;                           // id of row i0 + lane, one tile ahead
         const bool mine = (int)threadIdx.x < TQ;
         const auto issue = [&](int t, char *to) {
             const int i0 = t * TQ, rows = min(TQ, p.sq - i0);
@@ -301,11 +312,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
             if (mine) {
                 r_lse = stats[i0 + threadIdx.x];
                 r_delta = stats[p.sq_pad + i0 + threadIdx.x];
-                if (p.docs != nullptr) r_id = (int)threadIdx.x < rows ? ids[i0 + off + threadIdx.x] : -1;
             }
+            if (p.docs != nullptr) next_id = lane < rows ? ids[i0 + off + lane] : -1;
         };
         const auto put = [&](int to) {
-            if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; lds_id[to][threadIdx.x] = r_id; }
+            if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; }
         };
         TileWalk walk;
         walk.start(lo / TQ, (p.sq + TQ - 1) / TQ);
@@ -317,9 +328,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
             const int i0 = tile * TQ;
             char *lds_q = lds + buf * 2 * kTileBytes, *lds_g = lds_q + kTileBytes;
             const float *lse_of = lds_stat[buf][0], *delta_of = lds_stat[buf][1];
-            const int *id_of = lds_id[buf];
             const int next = walk.next(look);
             FD::wait();
+            place_id = next_id;
             __syncthreads();
             buf ^= 1;
             if (next >= 0) issue(next, lds + buf * 2 * kTileBytes);
@@ -329,32 +340,43 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
                 __syncthreads();
             }
             if (!skip) {
-                const int lim = first - i0 - 4 * half;
+                Seen seen;
+                if (!full) {
+                    uint64_t see = ~low_bits(first - i0);
+                    if (p.docs != nullptr) see &= same_id(place_id, id);
+                    seen = seen_from(see);
+                }
                 const float at_row = (float)(i0 + off + 4 * half - key);
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++) {
                     fx16 s = {}, dp = {};
+                    {   // fragments of q and dout, read up to four steps ahead of their products
+                        constexpr int W = C < 4 ? C : 4;
+                        frag qf[W], gf[W];
 #pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        s = AT::mma(TL::rows(lds_q, at_lane, 32 * qb, c), kf[c], s);
-                        dp = AT::mma(TL::rows(lds_g, at_lane, 32 * qb, c), vf[c], dp);
+                        for (int i = 0; i < W; i++) { qf[i] = TL::rows(lds_q, at_lane, 32 * qb, i); gf[i] = TL::rows(lds_g, at_lane, 32 * qb, i); }
+                        FLK_KEEP_ORDER();
+#pragma unroll
+                        for (int c = 0; c < C; c++) {
+                            s = AT::mma(qf[c % W], kf[c], s);
+                            dp = AT::mma(gf[c % W], vf[c], dp);
+                            if (c + W < C) { qf[c % W] = TL::rows(lds_q, at_lane, 32 * qb, c + W); gf[c % W] = TL::rows(lds_g, at_lane, 32 * qb, c + W); }
+                            FLK_KEEP_ORDER();
+                        }
                     }
+                    // fragments of dout and q across the rows, read before the weights are formed
+                    constexpr int F = ST * DB, W2 = F < 8 ? F : 8;
+                    frag gt[W2], qt[W2];
+#pragma unroll
+                    for (int i = 0; i < W2; i++) {
+                        gt[i] = TL::cols(lds_g, at_lane, 32 * qb + AT::KS * (i / DB), i % DB);
+                        qt[i] = TL::cols(lds_q, at_lane, 32 * qb + AT::KS * (i / DB), i % DB);
+                    }
+                    FLK_KEEP_ORDER();
 #pragma unroll
                     for (int g4 = 0; g4 < 4; g4++) {
                         const int a = 32 * qb + 8 * g4 + 4 * half;
                         const fx4 lse = *(const fx4 *)(lse_of + a), delta = *(const fx4 *)(delta_of + a);
-                        bool hide[4];
-                        if (!full) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) hide[i] = 32 * qb + 8 * g4 + i < lim;
-                            if (p.docs != nullptr) {
-                                const int4 t = *(const int4 *)(id_of + a);
-                                hide[0] |= t.x != id;
-                                hide[1] |= t.y != id;
-                                hide[2] |= t.z != id;
-                                hide[3] |= t.w != id;
-                            }
-                        }
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int r = 4 * g4 + i;
@@ -364,19 +386,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
                             g = e * (dp[r] - delta[i]);
                             if constexpr ((MOD & kCap) != 0) g *= grad;
                             if (!whole) e = __builtin_fmaf(delta[i], 0.f, e);
-                            if (!full) { e = hide[i] ? 0.f : e; g = hide[i] ? 0.f : g; }
+                            if (!full) { e = seen.or_zero(e, qb, r); g = seen.or_zero(g, qb, r); }
                             s[r] = e;
                             dp[r] = g;
                         }
                     }
 #pragma unroll
-                    for (int st = 0; st < ST; st++) {
-                        const frag pf = pack<T>(s, st), sf = pack<T>(dp, st);
-#pragma unroll
-                        for (int db = 0; db < DB; db++) {
-                            dv[db] = AT::mma(TL::cols(lds_g, at_lane, 32 * qb + AT::KS * st, db), pf, dv[db]);
-                            dk[db] = AT::mma(TL::cols(lds_q, at_lane, 32 * qb + AT::KS * st, db), sf, dk[db]);
+                    for (int i = 0; i < F; i++) {
+                        const frag pf = pack<T>(s, i / DB), sf = pack<T>(dp, i / DB);
+                        dv[i % DB] = AT::mma(gt[i % W2], pf, dv[i % DB]);
+                        dk[i % DB] = AT::mma(qt[i % W2], sf, dk[i % DB]);
+                        if (i + W2 < F) {
+                            gt[i % W2] = TL::cols(lds_g, at_lane, 32 * qb + AT::KS * ((i + W2) / DB), (i + W2) % DB);
+                            qt[i % W2] = TL::cols(lds_q, at_lane, 32 * qb + AT::KS * ((i + W2) / DB), (i + W2) % DB);
                         }
+                        FLK_KEEP_ORDER();
                     }
                 }
             }

@@ -77,6 +77,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
             if (!full) bad |= any_nonfinite<T>(rv[n]);
         }
         const bool careful = !full && __any(bad);
+        if (careful) {                                             // clear them for the product, and add what they do to it below
+#pragma unroll
+            for (int n = 0; n < N; n++) clean<T>(lds_v + (n * 64 + lane) * 16);
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (tile + 4 < tile_hi) fetch(tile + 4);
@@ -108,20 +112,6 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
 #pragma unroll
         for (int i = 0; i < 16; i++) sum[i & 3] += s[i];
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (careful) {
-            fx16 w = s, x[DB];                                     // through copies, so that s and o stay in registers elsewhere
-#pragma unroll
-            for (int db = 0; db < DB; db++) x[db] = o[db];
-            spread_nonfinite<T, DP, 1, DB>(lds_v, &w, x);
-#pragma unroll
-            for (int db = 0; db < DB; db++) o[db] = x[db];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int n = 0; n < N; n++) clean<T>(lds_v + (n * 64 + lane) * 16);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
 #pragma unroll
         for (int st = 0; st < ST; st++) {
             const frag pf = pack<T>(s, st);
@@ -130,6 +120,14 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                 const frag vf = TL::cols(lds_v, at_lane, AT::KS * st, db);
                 o[db] = AT::mma(vf, pf, o[db]);
             }
+        }
+        if (careful) {
+            fx16 w = s, x[DB];
+#pragma unroll
+            for (int db = 0; db < DB; db++) x[db] = o[db];
+            spread_nonfinite<T, 1, DB>(vbase + k0 * p.vs.s, p.vs.s, len - k0, p.dv_d, &w, x);
+#pragma unroll
+            for (int db = 0; db < DB; db++) o[db] = x[db];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();

@@ -34,7 +34,7 @@ constexpr int kDocBlock = 32;              // positions one entry of the documen
 template <typename T> struct AttnType;
 template <> struct AttnType<float> {
     typedef fx4 frag;
-    static constexpr int E = 4, KS = 8, kTile = 32;
+    static constexpr int E = 4, KS = 8, kTile = 32, M = 4, R = 4;   // M, R: matrix instructions and cross-row reads a fragment
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) {
 #pragma unroll
         for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
@@ -44,12 +44,12 @@ template <> struct AttnType<float> {
 };
 template <> struct AttnType<f16_t> {
     typedef hx8 frag;
-    static constexpr int E = 8, KS = 16, kTile = 64;
+    static constexpr int E = 8, KS = 16, kTile = 64, M = 1, R = 2;
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct AttnType<bf16_t> {
     typedef bx8 frag;
-    static constexpr int E = 8, KS = 16, kTile = 64;
+    static constexpr int E = 8, KS = 16, kTile = 64, M = 1, R = 2;
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
@@ -144,22 +144,24 @@ template <typename T> __device__ __forceinline__ void clean(char *at) {
         if (!(__builtin_fabsf((float)x.t[i]) < kInf)) x.t[i] = (T)0.f;
     *(ux4 *)at = x.u;
 }
-// What they add to the rows that see them: value (row, c) of a tile of TK rows for every output column this lane holds, where the
-// row's weight is not zero.  w[kb][r]: weights of key 32 kb + 8 (r / 4) + 4 half + r % 4.  Rare, and not made to be fast.
-template <typename T, int DP, int KB, int DB>
-__device__ __noinline__ void spread_nonfinite(const char *tile, const fx16 *w, fx16 *o) {
-    typedef Tile<T, DP> TL;
+// What they add to the rows that see them: value (key, c), read again from memory, for every output column c this lane holds,
+// where the row's weight is not zero.  w[kb][r]: weights of key 32 kb + 8 (r / 4) + 4 half + r % 4.  Rare, and not made to be
+// fast; called with copies, so that weights and output stay in registers elsewhere.
+template <typename T, int KB, int DB>
+__device__ __noinline__ void spread_nonfinite(const T *rows, int64_t stride, int n, int d, const fx16 *w, fx16 *o) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    for (int key = 0; key < 32 * KB; key++) {
-        const ux4 mine = lane < TL::NC ? *(const ux4 *)(tile + TL::at(key, lane)) : ux4{0, 0, 0, 0};
-        if (!__any(any_nonfinite<T>(mine))) continue;
+    for (int key = 0; key < min(n, 32 * KB); key++) {
+        const T *row = rows + key * stride;
+        bool bad = false;
+        for (int c = lane; c < d; c += 64) bad |= !(__builtin_fabsf((float)row[c]) < kInf);
+        if (!__any(bad)) continue;
         float x = w[key >> 5][4 * (key >> 3 & 3) + (key & 3)];
         const float y = __shfl_xor(x, 32, 64);
         x = (key >> 2 & 1) == half ? x : y;
         for (int db = 0; db < DB; db++)
             for (int r = 0; r < 16; r++) {
                 const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                const float v = (float)*(const T *)(tile + TL::at(key, c / AttnType<T>::E) + c % AttnType<T>::E * (int)sizeof(T));
+                const float v = c < d ? (float)row[c] : 0.f;
                 if (x != 0.f && !(__builtin_fabsf(v) < kInf)) o[db][r] += v;
             }
     }
@@ -253,7 +255,8 @@ template <typename T, int DP, int TR> struct Feed {
             }
         }
     }
-    static __device__ __forceinline__ void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    // (the builtin, which the compiler counts: it would wait again for whatever it takes to be still on its way)
+    static __device__ __forceinline__ void wait() { __builtin_amdgcn_s_waitcnt(0x0f70); asm volatile("" ::: "memory"); }
     static __device__ __forceinline__ void clean_share(char *tile) {
 #pragma unroll
         for (int n = 0; n < N; n++) clean<T>(tile + (n * kAttnThreads + threadIdx.x) * 16);
@@ -306,6 +309,39 @@ template <typename T, int MOD> struct Score {
     }
     static constexpr float kGrad = kHasCap && !kWide ? 4.f : 1.f;   // what `grad` leaves to the end
 };
+
+// Nothing is moved across it: left to itself, the compiler reads every fragment right before its use and waits for it.
+#define FLK_KEEP_ORDER() __builtin_amdgcn_sched_barrier(0)
+
+// Which of a tile's 64 places this lane's row (or key) sees, one bit each.  Bit 8 g + 4 half + i of a block of 32 belongs to
+// accumulator register 4 g + i, so the mask is shifted by 4 half once and every register asks for a fixed bit.
+struct Seen {
+    unsigned w[2];
+    // all ones where register r of block kb is seen
+    __device__ __forceinline__ int bits(int kb, int r) const { return (int)(w[kb] << (31 - (8 * (r >> 2) + (r & 3)))) >> 31; }
+    __device__ __forceinline__ float or_inf(float x, int kb, int r) const {        // x, or -inf where it is hidden
+        const int m = bits(kb, r);
+        return __builtin_bit_cast(float, (__builtin_bit_cast(int, x) & m) | ((int)0xff800000 & ~m));
+    }
+    __device__ __forceinline__ float or_zero(float x, int kb, int r) const { return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & bits(kb, r)); }
+};
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+// The places whose id (place l's in lane l) is this lane's: one round for every different id among the lanes, which are few.
+__device__ __forceinline__ uint64_t same_id(int place_id, int id) {
+    uint64_t m = 0, todo = __ballot(id >= 0);
+    while (todo != 0) {
+        const int now = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+        const uint64_t at = __ballot(place_id == now);
+        const bool mine = id == now;
+        m = mine ? at : m;
+        todo &= ~__ballot(mine);
+    }
+    return m;
+}
+__device__ __forceinline__ Seen seen_from(uint64_t m) {
+    m >>= 4 * (threadIdx.x >> 5 & 1);
+    return {{(unsigned)m, (unsigned)(m >> 32)}};
+}
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 __device__ __forceinline__ int wave_min(int x) {

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
         qf[c] = x.f;
     }
 
-    // documents: this row's id (no key has -2) and the span of the wave's and of the workgroup's rows
+    // documents: this row's id (negative: sees nothing) and the span of the wave's and of the workgroup's rows
     int id = 0;
     int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
         const int raw = live ? ids[pos] : -1;
         span = {wave_min(raw), wave_max(raw)};
         if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
-        id = raw < 0 ? -2 : raw;
+        id = raw;
         __syncthreads();
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
@@ -91,36 +91,57 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
     for (int db = 0; db < DB; db++) o[db] = fx16{};
     float m = -kInf, l = 0.f;                                      // m in units of log 2
 
+    int place_id = -1, next_id = -1;                               // id of key k0 + lane, one tile ahead
+    const auto id_at = [&](int t) {
+        const int k = t * TK + lane;
+        return lane < TK && k < p.sk ? ids[k] : -1;
+    };
     int buf = 0, tile = walk.next(look);
     bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
     if (tile >= 0) {
         feed_k.issue(lds, tile * TK, min(TK, p.sk - tile * TK));
         feed_v.issue(lds + kTileBytes, tile * TK, min(TK, p.sk - tile * TK));
+        if (p.docs != nullptr) next_id = id_at(tile);
     }
     while (tile >= 0) {
         const int k0 = tile * TK;
-        const char *lds_k = lds + buf * 2 * kTileBytes, *lds_v = lds_k + kTileBytes;
+        char *lds_k = lds + buf * 2 * kTileBytes, *lds_v = lds_k + kTileBytes;
         const int next = walk.next(look);
         FD::wait();
+        place_id = next_id;
         __syncthreads();                                           // this tile is there, the one before has been read
         buf ^= 1;
         if (next >= 0) {
             feed_k.issue(lds + buf * 2 * kTileBytes, next * TK, min(TK, p.sk - next * TK));
             feed_v.issue(lds + buf * 2 * kTileBytes + kTileBytes, next * TK, min(TK, p.sk - next * TK));
+            if (p.docs != nullptr) next_id = id_at(next);
         }
         bool careful = false;
         if (!whole) {
             if (FD::nonfinite(lds_v)) lds_bad = tile;
             __syncthreads();
             careful = lds_bad == tile;
+            if (careful) {                                         // clear them for the product, and add what they do to it below
+                FD::clean_share(lds_v);
+                __syncthreads();
+            }
         }
-        fx16 s[KB];
         if (!skip) {
+            fx16 s[KB];
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                s[kb] = fx16{};
+            for (int kb = 0; kb < KB; kb++) s[kb] = fx16{};
+            {   // fragments of the keys, read up to eight ahead of their products
+                constexpr int n = KB * C, W = n < 8 ? n : 8;
+                frag kf[W];
 #pragma unroll
-                for (int c = 0; c < C; c++) s[kb] = AT::mma(TL::rows(lds_k, at_lane, 32 * kb, c), qf[c], s[kb]);
+                for (int i = 0; i < W; i++) kf[i] = TL::rows(lds_k, at_lane, 32 * (i % KB), i / KB);
+                FLK_KEEP_ORDER();
+#pragma unroll
+                for (int i = 0; i < n; i++) {
+                    s[i % KB] = AT::mma(kf[i % W], qf[i / KB], s[i % KB]);
+                    if (i + W < n) kf[i % W] = TL::rows(lds_k, at_lane, 32 * ((i + W) % KB), (i + W) / KB);
+                    FLK_KEEP_ORDER();
+                }
             }
             if constexpr (!kLate) {
                 const float at = (float)(pos - k0 - 4 * half);
@@ -132,24 +153,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
                         s[kb][r] = score(s[kb][r], at - (float)(32 * kb + 8 * (r >> 2) + (r & 3)), grad);
                     }
             }
+            Seen seen;
             if (!full) {
-                const int lim = last - k0 - 4 * half;
+                uint64_t see = low_bits(last + 1 - k0);
+                if (p.docs != nullptr) see &= same_id(place_id, id);
+                seen = seen_from(see);
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[kb][r] = 32 * kb + 8 * (r >> 2) + (r & 3) <= lim ? s[kb][r] : -kInf;
-                if (p.docs != nullptr) {
-#pragma unroll
-                    for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            const int4 t = *(const int4 *)(ids + min(k0 + 32 * kb, (p.doc_blocks - 1) * kDocBlock) + 8 * g + 4 * half);
-                            s[kb][4 * g] = t.x == id ? s[kb][4 * g] : -kInf;
-                            s[kb][4 * g + 1] = t.y == id ? s[kb][4 * g + 1] : -kInf;
-                            s[kb][4 * g + 2] = t.z == id ? s[kb][4 * g + 2] : -kInf;
-                            s[kb][4 * g + 3] = t.w == id ? s[kb][4 * g + 3] : -kInf;
-                        }
-                }
+                    for (int r = 0; r < 16; r++) s[kb][r] = seen.or_inf(s[kb][r], kb, r);
             }
             float top = -kInf;
 #pragma unroll
@@ -167,45 +179,55 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
                 for (int db = 0; db < DB; db++) o[db] *= a;
             }
             const float base_m = m == -kInf ? 0.f : m;
+            // Weights and their product with the values.  The first fragments of the values are on their way before the first
+            // weights are formed; the weights of the next 32 keys are formed between the products of the present ones.
             float sum[4] = {0.f, 0.f, 0.f, 0.f};                   // short chains: long ones would cost float data digits
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    if constexpr (MOD == kPlain) s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], score.unit, -base_m));
-                    else if constexpr (!kLate) s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r] - base_m);
-                    else {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score.r(s[kb][r]), -2.f * score.out, score.out - base_m));
-                        s[kb][r] = full || s[kb][r] != -kInf ? e : 0.f;
-                    }
-                    sum[r & 3] += s[kb][r];
+            const auto weight = [&](int kb, int r) {
+                float e;
+                if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], score.unit, -base_m));
+                else if constexpr (!kLate) e = __builtin_amdgcn_exp2f(s[kb][r] - base_m);
+                else {
+                    e = __builtin_amdgcn_exp2f(__builtin_fmaf(score.r(s[kb][r]), -2.f * score.out, score.out - base_m));
+                    e = full || s[kb][r] != -kInf ? e : 0.f;
                 }
+                s[kb][r] = e;
+                sum[r & 3] += e;
+            };
+            constexpr int F = ST * DB, EX = (16 + F - 1) / F;
+            frag vf[F], pf[ST];
+#pragma unroll
+            for (int i = 0; i < F; i++) vf[i] = TL::cols(lds_v, at_lane, AT::KS * (i / DB), i % DB);
+            FLK_KEEP_ORDER();
+#pragma unroll
+            for (int r = 0; r < 16; r++) weight(0, r);
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+                for (int st = 0; st < ST; st++) pf[st] = pack<T>(s[kb], st);
+                FLK_KEEP_ORDER();
+#pragma unroll
+                for (int i = 0; i < F; i++) {
+                    o[i % DB] = AT::mma(vf[i], pf[i / DB], o[i % DB]);
+                    if (kb + 1 < KB) {
+                        vf[i] = TL::cols(lds_v, at_lane, 32 * (kb + 1) + AT::KS * (i / DB), i % DB);
+#pragma unroll
+                        for (int r = i * EX; r < (i + 1) * EX; r++)
+                            if (r < 16) weight(kb + 1, r);
+                    }
+                    FLK_KEEP_ORDER();
+                }
+            }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-        if (careful) {
-            if (!skip) {                                           // through copies, so that s and o stay in registers elsewhere
+            if (careful) {
                 fx16 w[KB], x[DB];
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++) w[kb] = s[kb];
 #pragma unroll
                 for (int db = 0; db < DB; db++) x[db] = o[db];
-                spread_nonfinite<T, DP, KB, DB>(lds_v, w, x);
+                spread_nonfinite<T, KB, DB>(feed_v.base + k0 * feed_v.stride, feed_v.stride, p.sk - k0, p.dv_d, w, x);
 #pragma unroll
                 for (int db = 0; db < DB; db++) o[db] = x[db];
             }
-            __syncthreads();
-            FD::clean_share(lds + (buf ^ 1) * 2 * kTileBytes + kTileBytes);
-            __syncthreads();
-        }
-        if (!skip) {
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                for (int st = 0; st < ST; st++) {
-                    const frag pf = pack<T>(s[kb], st);
-#pragma unroll
-                    for (int db = 0; db < DB; db++) o[db] = AT::mma(TL::cols(lds_v, at_lane, 32 * kb + AT::KS * st, db), pf, o[db]);
-                }
         }
         tile = next;
         whole = walk.is_whole;
