@@ -166,31 +166,62 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     }
 }
 
-// out from the parts of `splits` workgroups, one thread a value
-template <typename T>
-__global__ void __launch_bounds__(kAttnThreads) attention_cached_join_kernel(CachedArgs p) {
-    const int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x;
-    if (i >= (int64_t)p.b * p.t * p.hq * p.dv_d) return;
-    const int64_t row = i / p.dv_d, c = i % p.dv_d;
-    const float *ml = p.part_ml + row * p.splits * 2, *po = p.part_o + row * p.splits * p.dv_d + c;
+// out from the parts of `splits` workgroups: a workgroup a row.  The parts' shares first, one thread each; then threads in groups
+// that hold the row's values add the parts, every group each `groups`-th one, and the groups' sums meet in LDS.
+constexpr int kMaxSplits = 256;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) attention_cached_join_kernel(CachedArgs p) {
+    __shared__ float share[kMaxSplits], sums[THREADS], lds_top[THREADS / 64], lds_sum[THREADS / 64];
+    const int64_t row = blockIdx.x;
+    const float *ml = p.part_ml + row * p.splits * 2, *po = p.part_o + row * p.splits * p.dv_d;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float top = -kInf;
-    for (int s = 0; s < p.splits; s++) top = fmaxf(top, ml[2 * s]);
-    float x = 0.f, sum = 0.f;
-    for (int s = 0; s < p.splits; s++) {
-        if (ml[2 * s] == -kInf && ml[2 * s + 1] == 0.f) continue;
-        const float a = ml[2 * s] == -kInf ? 1.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
-        x += a * po[(int64_t)s * p.dv_d];
-        sum += a * ml[2 * s + 1];
+    for (int s = threadIdx.x; s < p.splits; s += THREADS) top = fmaxf(top, ml[2 * s]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (lane == 0) lds_top[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) top = fmaxf(top, lds_top[w]);
+    float sum = 0.f;
+    for (int s = threadIdx.x; s < p.splits; s += THREADS) {
+        const float m = ml[2 * s], l = ml[2 * s + 1];
+        // a part that saw nothing has no share; one whose scores were all NaN has a maximum of -inf and a sum of NaN
+        const float a = m == -kInf ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
+        share[s] = a;
+        sum += a * l;
     }
-    ((T *)p.out)[i] = (T)(sum == 0.f ? 0.f : x / sum);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) lds_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) sum += lds_sum[w];
+    int width = 32;
+    while (width < p.dv_d) width *= 2;                             // at most 128, the padded head
+    const int c = threadIdx.x % width, group = threadIdx.x / width, groups = THREADS / width;
+    float x = 0.f;
+    if (c < p.dv_d) {
+#pragma unroll 8
+        for (int s = group; s < p.splits; s += groups)
+            if (share[s] != 0.f) x += share[s] * po[(int64_t)s * p.dv_d + c];
+    }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    if (group != 0 || c >= p.dv_d) return;
+    x = 0.f;
+    for (int g = 0; g < groups; g++) x += sums[g * width + c];
+    ((T *)p.out)[row * p.dv_d + c] = (T)(sum == 0.f ? 0.f : x / sum);
 }
 
 template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.blocks_r * a.splits));
     FLK_ATTN_LAUNCH(attention_cached_kernel, grid)
     if (a.splits > 1) {
-        const int64_t n = (int64_t)a.b * a.t * a.hq * a.dv_d;
-        hipLaunchKernelGGL((attention_cached_join_kernel<T>), dim3((unsigned)((n + kAttnThreads - 1) / kAttnThreads)), dim3(kAttnThreads), 0, st, a);
+        const dim3 rows((unsigned)((int64_t)a.b * a.t * a.hq));
+        if (a.splits > 16) hipLaunchKernelGGL((attention_cached_join_kernel<T, 1024>), rows, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL((attention_cached_join_kernel<T, 128>), rows, dim3(128), 0, st, a);
         FLK_LAUNCH_CHECK("attention_cached_join_kernel");
     }
     return FLK_OK;
