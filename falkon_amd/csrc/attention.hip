@@ -51,10 +51,11 @@ static bool attn_dtype(int dtype) { return dtype == FLK_F32 || dtype == FLK_F16 
 static int padded_d(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 static bool rows_aligned(const void *p, const AttnStride &s, int64_t d, int es) {
     const int64_t e = 16 / es;
     if (s.s > ((int64_t)1 << 23) || s.s < 0) return false;        // a tile's offsets are 32 bits wide
-    return ((uintptr_t)p & 15) == 0 && s.b % e == 0 && s.s % e == 0 && s.h % e == 0 && d % e == 0;
+    return aligned16(p) && s.b % e == 0 && s.s % e == 0 && s.h % e == 0 && d % e == 0;
 }
 
 // document spans, then ids
@@ -175,7 +176,7 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
     a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)cdiv(sk, kDocBlock);
     place_docs(a, workspace);
     const int es = elem_size(dtype);
-    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) && aligned16(out) && aligned16(a.rest);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);
@@ -222,7 +223,7 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     a.dkv_part = (float *)ws;
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) &&
-            rows_aligned(out, a.vs, dv, es) && rows_aligned(a.rest, a.vs, dv, es) && rows_aligned(dout, a.dos, dv, es);
+            rows_aligned(dout, a.dos, dv, es) && aligned16(out) && aligned16(a.rest) && aligned16(dq) && aligned16(dk) && aligned16(dv_out);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);

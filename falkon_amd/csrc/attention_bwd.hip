@@ -213,15 +213,11 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         if (threadIdx.x == 0)
             p.dslopes_part[((int64_t)h * p.b + b) * tiles_q + tile_q] = (lds_sum[0] + lds_sum[1]) + (lds_sum[2] + lds_sum[3]);
     }
-    if (!live || p.dq == nullptr) return;
-    T *out = (T *)p.dq + (((int64_t)b * p.sq + row) * p.hq + h) * p.d;
-#pragma unroll
-    for (int db = 0; db < DB; db++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (c < p.d) out[c] = (T)(acc[db][r] * (p.scale * score.kGrad));
-        }
+    if (p.dq == nullptr) return;
+    __syncthreads();
+    const float unscale = p.scale * score.kGrad;
+    store_rows<T, DP>(lds + wave * 32 * TL::RB, [&](int db, int r) { return acc[db][r] * unscale; },
+                      (T *)p.dq + (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, (int64_t)p.hq * p.d, p.sq - (i0 + wave * 32), p.d, p.vec);
 }
 
 template <typename T, int DP, int MOD>
@@ -411,29 +407,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
             skip = walk.is_skip;
         }
     }
-    if (!live) return;
-    const int64_t at_k = (((int64_t)b * p.sk + key) * p.hk + hk) * p.d, at_v = (((int64_t)b * p.sk + key) * p.hk + hk) * p.dv_d;
+    __syncthreads();
+    const float unscale = p.scale * Score<T, MOD>::kGrad;
+    const int rows = p.sk - k_lo;
+    const int64_t line = (int64_t)b * p.sk + k_lo, at_k = (line * p.hk + hk) * p.d, at_v = (line * p.hk + hk) * p.dv_d;
+    const int64_t row_k = (int64_t)p.hk * p.d, row_v = (int64_t)p.hk * p.dv_d;
     if (p.splits == 1) {
-        T *ok = (T *)p.dk + at_k, *ov = (T *)p.dv + at_v;
-#pragma unroll
-        for (int db = 0; db < DB; db++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (c < p.d) ok[c] = (T)(dk[db][r] * (p.scale * Score<T, MOD>::kGrad));
-                if (c < p.dv_d) ov[c] = (T)dv[db][r];
-            }
+        char *mine = lds + wave * 32 * TL::RB;
+        store_rows<T, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, (T *)p.dk + at_k, row_k, rows, p.d, p.vec);
+        store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r]; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec);
     } else {                                                       // parts in float, added by attention_join_kernel
-        const int64_t nk = (int64_t)p.b * p.sk * p.hk * p.d, nv = (int64_t)p.b * p.sk * p.hk * p.dv_d;
-        float *ok = p.dkv_part + split * nk + at_k, *ov = p.dkv_part + p.splits * nk + split * nv + at_v;
-#pragma unroll
-        for (int db = 0; db < DB; db++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (c < p.d) ok[c] = dk[db][r] * (p.scale * Score<T, MOD>::kGrad);
-                if (c < p.dv_d) ov[c] = dv[db][r];
-            }
+        const int64_t nk = (int64_t)p.b * p.sk * row_k, nv = (int64_t)p.b * p.sk * row_v;
+        char *mine = lds + wave * 32 * Tile<float, DP>::RB;
+        store_rows<float, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, p.dkv_part + split * nk + at_k, row_k, rows, p.d, p.d % 4 == 0);
+        store_rows<float, DP>(mine, [&](int db, int r) { return dv[db][r]; }, p.dkv_part + p.splits * nk + split * nv + at_v, row_v, rows, p.dv_d,
+                              p.d % 4 == 0 && p.dv_d % 4 == 0);
     }
 }
 

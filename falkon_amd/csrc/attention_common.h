@@ -270,6 +270,41 @@ template <typename T, int DP, int TR> struct Feed {
     }
 };
 
+// A wave's 32 rows of results, which lie in registers four values at a time (value 32 db + 8 g + 4 half + i of row lane % 32 in
+// x[db][4 g + i]), to memory in whole rows: through 32 rows of a tile in LDS that belong to this wave alone.  Written from the
+// registers, a row of 128 16-bit values would be 64 stores of two bytes (2048 workgroups: 80 us for nothing but that).
+// part(db, r): the value to write.
+template <typename T, int DP, typename Part>
+__device__ __forceinline__ void store_rows(char *lds, Part part, T *out, int64_t stride, int rows, int d, int vec) {
+    typedef Tile<T, DP> TL;
+    constexpr int E = AttnType<T>::E, NC = TL::NC;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");         // what was read there before has been read
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int db = 0; db < DP / 32; db++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int c = 32 * db + 8 * g + 4 * half;
+            struct alignas(4 * sizeof(T)) { T t[4]; } x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.t[i] = (T)part(db, 4 * g + i);
+            *(decltype(x) *)(lds + TL::at(lane & 31, c / E) + c % E * (int)sizeof(T)) = x;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+    for (int i = lane; i < 32 * NC; i += 64) {
+        const int row = i / NC, c = i % NC;
+        if (row >= rows || c * E >= d) continue;
+        const char *from = lds + TL::at(row, c);
+        T *to = out + row * stride + c * E;
+        if (vec) *(ux4 *)to = *(const ux4 *)from;
+        else
+            for (int j = 0; j < E && c * E + j < d; j++) to[j] = ((const T *)from)[j];
+    }
+}
+
 // What happens to the scores before the softmax.  A scale that is not positive goes with kDecay, whose rows look for their
 // maximum among the finished scores.
 constexpr int kPlain = 0, kCap = 1, kDecay = 2, kCapDecay = 3;

@@ -235,22 +235,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs
         skip = walk.is_skip;
     }
     l += other_half(l);
-    if (!live) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;                    // a row that sees nothing is zero
-    const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
-    T *orow = (T *)p.o + at, *rest = p.rest != nullptr ? (T *)p.rest + at : nullptr;
 #pragma unroll
-    for (int db = 0; db < DB; db++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (c < p.dv_d) {
-                const float x = o[db][r] * inv;
-                const T y = (T)x;
-                orow[c] = y;
-                if (rest != nullptr) rest[c] = (T)(x - (float)y);
-            }
-        }
+    for (int db = 0; db < DB; db++) o[db] *= inv;
+    const int64_t row_o = (int64_t)p.hq * p.dv_d, at = (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.dv_d;
+    const int rows = p.sq - (i0 + wave * 32);
+    __syncthreads();
+    char *mine = lds + wave * 32 * TL::RB;
+    store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r]; }, (T *)p.o + at, row_o, rows, p.dv_d, p.vec);
+    if (p.rest != nullptr)
+        store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r] - (float)(T)o[db][r]; }, (T *)p.rest + at, row_o, rows, p.dv_d, p.vec);
+    if (!live) return;
     if (half == 0 && p.lse != nullptr)
         p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : m * kLn2 + __logf(l);
 }
