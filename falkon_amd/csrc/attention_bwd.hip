@@ -220,8 +220,11 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                       (T *)p.dq + (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, (int64_t)p.hq * p.d, p.sq - (i0 + wave * 32), p.d, p.vec);
 }
 
+// Whether the dk / dv kernel's fragments and sums (keys, values, dk and dv of 32 keys in registers) leave room for one wave a SIMD only
+template <typename T, int DP> constexpr bool kAlone = sizeof(T) == 4 ? DP >= 64 : DP > 64;
+
 template <typename T, int DP, int MOD>
-__global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attention_dkv_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
@@ -336,67 +339,111 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attention_dkv_kernel(AttnArgs
                 __syncthreads();
             }
             if (!skip) {
-                Seen seen;
+                Seen seen = {{~0u, ~0u}};
                 if (!full) {
                     uint64_t see = ~low_bits(first - i0);
                     if (p.docs != nullptr) see &= same_id(place_id, id);
                     seen = seen_from(see);
                 }
                 const float at_row = (float)(i0 + off + 4 * half - key);
+                constexpr int kAhead = kAlone<T, DP> ? 4 : 2;         // steps that fragments are read ahead
+                constexpr int N = QB * C, W = N < kAhead ? N : kAhead, F = ST * DB, NF = QB * F, WF = NF < kAhead ? NF : kAhead;
+                frag qf[W], gf[W], gt[WF], qt[WF], pf, sf;
+                fx16 s[QB], dp[QB];
+                fx4 lse[4], delta[4];
+                const auto read_rows = [&](int n) {
+                    qf[n % W] = TL::rows(lds_q, at_lane, 32 * (n / C), n % C);
+                    gf[n % W] = TL::rows(lds_g, at_lane, 32 * (n / C), n % C);
+                };
+                const auto read_cols = [&](int n) {
+                    const int row = 32 * (n / F) + AT::KS * (n % F / DB);
+                    gt[n % WF] = TL::cols(lds_g, at_lane, row, n % DB);
+                    qt[n % WF] = TL::cols(lds_q, at_lane, row, n % DB);
+                };
+                const auto read_stats = [&](int qb, int g4) {
+                    lse[g4] = *(const fx4 *)(lse_of + 32 * qb + 8 * g4 + 4 * half);
+                    delta[g4] = *(const fx4 *)(delta_of + 32 * qb + 8 * g4 + 4 * half);
+                };
+                const auto scores = [&](int n) {                   // one step of the products behind scores and their gradients
+                    const int qb = n / C, c = n % C;
+                    s[qb] = AT::mma(qf[n % W], kf[c], c == 0 ? fx16{} : s[qb]);
+                    dp[qb] = AT::mma(gf[n % W], vf[c], c == 0 ? fx16{} : dp[qb]);
+                    if (n + W < N) read_rows(n + W);
+                };
+                const auto weight = [&](int qb, int r, bool masked) {
+                    const float li = lse[r >> 2][r & 3], de = delta[r >> 2][r & 3];
+                    float e, g, grad = 1.f;
+                    if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][r], score.unit, -li));
+                    else e = __builtin_amdgcn_exp2f(score(s[qb][r], at_row + (float)(32 * qb + 8 * (r >> 2) + (r & 3)), grad) - li);
+                    g = e * (dp[qb][r] - de);
+                    if constexpr ((MOD & kCap) != 0) g *= grad;
+                    if (masked) {
+                        e = seen.or_zero(__builtin_fmaf(de, 0.f, e), qb, r);
+                        g = seen.or_zero(g, qb, r);
+                    }
+                    s[qb][r] = e;
+                    dp[qb][r] = g;
+                };
+                const auto gradients = [&](int n) {                // one step of the gradients' products
+                    const int qb = n / F, i = n % F;
+                    if (i % DB == 0) { pf = pack<T>(s[qb], i / DB); sf = pack<T>(dp[qb], i / DB); }
+                    dv[i % DB] = AT::mma(gt[n % WF], pf, dv[i % DB]);
+                    dk[i % DB] = AT::mma(qt[n % WF], sf, dk[i % DB]);
+                    if (n + WF < NF) read_cols(n + WF);
+                };
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++) {
-                    fx16 s = {}, dp = {};
-                    {   // fragments of q and dout, read up to four steps ahead of their products
-                        constexpr int W = C < 4 ? C : 4;
-                        frag qf[W], gf[W];
+                for (int n = 0; n < W; n++) read_rows(n);
+                FLK_KEEP_ORDER();
+                if constexpr (kAlone<T, DP> && QB == 2) {
+                    // One wave a SIMD has to keep its matrix cores busy by itself: the weights of the first 32 rows are formed
+                    // between the score products of the second, and theirs between the gradient products of the first.  No
+                    // branch may stand between them, so every tile is masked (2 x 4096 positions, 32 heads of 128, causal: the whole
+                    // backward pass 1.37 ms with the steps one after the other, 1.23 ms so).
+                    constexpr int EC = (16 + C - 1) / C, EF = (16 + F - 1) / F;
 #pragma unroll
-                        for (int i = 0; i < W; i++) { qf[i] = TL::rows(lds_q, at_lane, 32 * qb, i); gf[i] = TL::rows(lds_g, at_lane, 32 * qb, i); }
+                    for (int c = 0; c < C; c++) { scores(c); FLK_KEEP_ORDER(); }
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; g4++) read_stats(0, g4);
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        scores(C + c);
+#pragma unroll
+                        for (int n = c * WF / C; n < (c + 1) * WF / C; n++) read_cols(n);
+#pragma unroll
+                        for (int r = c * EC; r < (c + 1) * EC; r++)
+                            if (r < 16) weight(0, r, true);
                         FLK_KEEP_ORDER();
-#pragma unroll
-                        for (int c = 0; c < C; c++) {
-                            s = AT::mma(qf[c % W], kf[c], s);
-                            dp = AT::mma(gf[c % W], vf[c], dp);
-                            if (c + W < C) { qf[c % W] = TL::rows(lds_q, at_lane, 32 * qb, c + W); gf[c % W] = TL::rows(lds_g, at_lane, 32 * qb, c + W); }
-                            FLK_KEEP_ORDER();
-                        }
                     }
-                    // fragments of dout and q across the rows, read before the weights are formed
-                    constexpr int F = ST * DB, W2 = F < 8 ? F : 8;
-                    frag gt[W2], qt[W2];
 #pragma unroll
-                    for (int i = 0; i < W2; i++) {
-                        gt[i] = TL::cols(lds_g, at_lane, 32 * qb + AT::KS * (i / DB), i % DB);
-                        qt[i] = TL::cols(lds_q, at_lane, 32 * qb + AT::KS * (i / DB), i % DB);
-                    }
-                    FLK_KEEP_ORDER();
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; g4++) {
-                        const int a = 32 * qb + 8 * g4 + 4 * half;
-                        const fx4 lse = *(const fx4 *)(lse_of + a), delta = *(const fx4 *)(delta_of + a);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r = 4 * g4 + i;
-                            float e, g, grad = 1.f;
-                            if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse[i]));
-                            else e = __builtin_amdgcn_exp2f(score(s[r], at_row + (float)(32 * qb + 8 * g4 + i), grad) - lse[i]);
-                            g = e * (dp[r] - delta[i]);
-                            if constexpr ((MOD & kCap) != 0) g *= grad;
-                            if (!whole) e = __builtin_fmaf(delta[i], 0.f, e);
-                            if (!full) { e = seen.or_zero(e, qb, r); g = seen.or_zero(g, qb, r); }
-                            s[r] = e;
-                            dp[r] = g;
-                        }
-                    }
+                    for (int g4 = 0; g4 < 4; g4++) read_stats(1, g4);
 #pragma unroll
                     for (int i = 0; i < F; i++) {
-                        const frag pf = pack<T>(s, i / DB), sf = pack<T>(dp, i / DB);
-                        dv[i % DB] = AT::mma(gt[i % W2], pf, dv[i % DB]);
-                        dk[i % DB] = AT::mma(qt[i % W2], sf, dk[i % DB]);
-                        if (i + W2 < F) {
-                            gt[i % W2] = TL::cols(lds_g, at_lane, 32 * qb + AT::KS * ((i + W2) / DB), (i + W2) % DB);
-                            qt[i % W2] = TL::cols(lds_q, at_lane, 32 * qb + AT::KS * ((i + W2) / DB), (i + W2) % DB);
+                        gradients(i);
+#pragma unroll
+                        for (int r = i * EF; r < (i + 1) * EF; r++)
+                            if (r < 16) weight(1, r, true);
+                        FLK_KEEP_ORDER();
+                    }
+#pragma unroll
+                    for (int i = F; i < NF; i++) { gradients(i); FLK_KEEP_ORDER(); }
+                } else {
+                    const bool masked = !(whole && full);
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++) {
+#pragma unroll
+                        for (int c = 0; c < C; c++) { scores(qb * C + c); FLK_KEEP_ORDER(); }
+                        if (qb == 0) {
+#pragma unroll
+                            for (int n = 0; n < WF; n++) read_cols(n);
                         }
                         FLK_KEEP_ORDER();
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            if (r % 4 == 0) read_stats(qb, r / 4);
+                            weight(qb, r, masked);
+                        }
+#pragma unroll
+                        for (int i = 0; i < F; i++) { gradients(qb * F + i); FLK_KEEP_ORDER(); }
                     }
                 }
             }
