@@ -33,12 +33,10 @@ HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
     # packed fp32 VALU ops are kept out of the generated code on purpose
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # keep MFMA accumulators in VGPRs: the epilogue reads every accumulator with VALU ops
+    "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     "-Wno-unused-command-line-argument",
 ]
-# keep MFMA accumulators in VGPRs: the epilogue reads every accumulator with VALU ops.  Not where the accumulators of one
-# wave (dk and dv of attention's backward pass) fill more than the half of the registers that VALU ops reach.
-MFMA_IN_VGPRS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-MFMA_ANYWHERE = ("attention_bwd.hip",)
 
 
 def _hipcc() -> str:
@@ -62,8 +60,7 @@ def _compile(job) -> str:
         if os.path.getmtime(obj) > max(os.path.getmtime(os.path.join(CSRC, src)), _headers_mtime()):
             return obj
     defines = [] if kf is None else [f"-DFLK_KF={kf}"]
-    form = [] if src in MFMA_ANYWHERE else MFMA_IN_VGPRS
-    cmd = [_hipcc(), *HIPCC_FLAGS, *form, *defines, "-c", os.path.join(CSRC, src), "-o", obj]
+    cmd = [_hipcc(), *HIPCC_FLAGS, *defines, "-c", os.path.join(CSRC, src), "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src} {' '.join(defines)}:\n{res.stderr}")

@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
     frag qf[C], gf[C];
     float delta = 0.f;
+    unsigned bits = 0;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         union { ux4 u; frag f; } x, g, o, e;
@@ -57,9 +58,12 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         e.u = load_chunk<T>((const T *)p.rest + at, 2 * c + half, p.dv_d, live && p.rest != nullptr, p.vec);
         qf[c] = x.f;
         gf[c] = g.f;
+        bits |= bad_bits<T>(x.u) | bad_bits<T>(g.u);
 #pragma unroll
         for (int i = 0; i < AT::E; i++) delta += (float)g.f[i] * ((float)o.f[i] + (float)e.f[i]);
     }
+    // a row with a NaN or an infinity in q or dout has gradients of NaN, and its delta says so to the other kernel
+    if (any_bad<T>(bits)) delta = __builtin_nanf("");
     delta += other_half(delta);
     // the statistics of this tile's rows, for both kernels; a row that sees nothing, or is none, has every p zero
     float lse = kInf;
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
             for (int kb = 0; kb < KB; kb++) {
                 fx16 s = {}, dp = {};
                 {   // fragments of keys and values, read up to four steps ahead of their products
-                    constexpr int W = C < 4 ? C : 4;
+                    constexpr int W = C < 4 ? C : sizeof(T) == 2 && DP > 96 ? 2 : 4;     // (as the registers allow)
                     frag kf[W], vf[W];
 #pragma unroll
                     for (int i = 0; i < W; i++) { kf[i] = TL::rows(lds_k, at_lane, 32 * kb, i); vf[i] = TL::rows(lds_v, at_lane, 32 * kb, i); }
@@ -164,10 +168,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                         FLK_KEEP_ORDER();
                     }
                 }
-                constexpr int F = ST * DB;
-                frag kt[F];
+                constexpr int F = ST * DB, WF = F < 4 ? F : 4;
+                frag kt[WF], ds;
 #pragma unroll
-                for (int i = 0; i < F; i++) kt[i] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * (i / DB), i % DB);
+                for (int i = 0; i < WF; i++) kt[i] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * (i / DB), i % DB);
                 FLK_KEEP_ORDER();
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
@@ -188,11 +192,13 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                     if constexpr ((MOD & kCap) != 0) g *= grad;
                     s[r] = g;
                 }
+                FLK_KEEP_ORDER();
 #pragma unroll
-                for (int st = 0; st < ST; st++) {
-                    const frag ds = pack<T>(s, st);
-#pragma unroll
-                    for (int db = 0; db < DB; db++) acc[db] = AT::mma(kt[st * DB + db], ds, acc[db]);
+                for (int i = 0; i < F; i++) {
+                    if (i % DB == 0) ds = pack<T>(s, i / DB);
+                    acc[i % DB] = AT::mma(kt[i % WF], ds, acc[i % DB]);
+                    if (i + WF < F) kt[i % WF] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * ((i + WF) / DB), (i + WF) % DB);
+                    FLK_KEEP_ORDER();
                 }
             }
         }
@@ -292,48 +298,71 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
 #pragma unroll
     for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
 
-    const int h_lo = p.group * split / p.splits, h_hi = p.group * (split + 1) / p.splits;
-    for (int hg = h_lo; hg < h_hi; hg++) {
-        const int h = hk * p.group + hg;
-        const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
-        const float *stats = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad;
-        FD feed_q, feed_g;
-        feed_q.init((const T *)p.q + b * p.qs.b + h * p.qs.h, p.qs.s, p.d, p.vec);
-        feed_g.init((const T *)p.dout + b * p.dos.b + h * p.dos.h, p.dos.s, p.dv_d, p.vec);
-        // a tile's statistics (padded to whole tiles of 128 rows) pass through registers of its first threads
-        float r_lse = 0.f, r_delta = 0.f;
-        int place_id = -1, next_id = -1;                           // id of row i0 + lane, one tile ahead
-        const bool mine = (int)threadIdx.x < TQ;
-        const auto issue = [&](int t, char *to) {
-            const int i0 = t * TQ, rows = min(TQ, p.sq - i0);
-            feed_q.issue(to, i0, rows);
-            feed_g.issue(to + kTileBytes, i0, rows);
-            if (mine) {
-                r_lse = stats[i0 + threadIdx.x];
-                r_delta = stats[p.sq_pad + i0 + threadIdx.x];
-            }
-            if (p.docs != nullptr) next_id = lane < rows ? ids[i0 + off + lane] : -1;
-        };
-        const auto put = [&](int to) {
-            if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; }
-        };
-        TileWalk walk;
-        walk.start(lo / TQ, (p.sq + TQ - 1) / TQ);
-        int buf = 0, tile = walk.next(look);
+    // the heads that share this key head, one after the other; the tiles to visit are the same for each
+    int head = p.group * split / p.splits;                         // of the tile on its way
+    const int head_end = p.group * (split + 1) / p.splits;
+    Score<T, MOD> score(p.scale, p.cap, 0.f);
+    FD feed_q, feed_g;
+    feed_q.init((const T *)p.q + b * p.qs.b + (hk * p.group + head) * p.qs.h, p.qs.s, p.d, p.vec);
+    feed_g.init((const T *)p.dout + b * p.dos.b + (hk * p.group + head) * p.dos.h, p.dos.s, p.dv_d, p.vec);
+    const float *stats = p.stats + ((int64_t)b * p.hq + hk * p.group + head) * 2 * p.sq_pad;
+    // a tile's statistics (padded to whole tiles of 128 rows) pass through registers of its first threads
+    float r_lse = 0.f, r_delta = 0.f;
+    int place_id = -1, next_id = -1;                               // id of row i0 + lane, one tile ahead
+    const bool mine = (int)threadIdx.x < TQ;
+    const auto issue = [&](int t, char *to) {
+        const int i0 = t * TQ, rows = min(TQ, p.sq - i0);
+        feed_q.issue(to, i0, rows);
+        feed_g.issue(to + kTileBytes, i0, rows);
+        if (mine) {
+            r_lse = stats[i0 + threadIdx.x];
+            r_delta = stats[p.sq_pad + i0 + threadIdx.x];
+        }
+        if (p.docs != nullptr) next_id = lane < rows ? ids[i0 + off + lane] : -1;
+    };
+    const auto put = [&](int to) {
+        if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; }
+    };
+    const int tile_lo = lo / TQ, tile_end = (p.sq + TQ - 1) / TQ;
+    TileWalk walk, again;
+    walk.start(tile_lo, tile_end);
+    int tile = walk.next(look);
+    again = walk;                                                  // the first 64 tiles as they were found
+    const int first_tile = tile;
+    const bool first_whole = walk.is_whole, first_full = walk.is_full, first_skip = walk.is_skip;
+    const auto advance = [&]() {
+        const int t = walk.next(look);
+        if (t >= 0 || head + 1 >= head_end) return t;
+        head++;
+        feed_q.base += p.qs.h;
+        feed_g.base += p.dos.h;
+        stats += 2 * p.sq_pad;
+        walk = again;
+        walk.is_whole = first_whole;
+        walk.is_full = first_full;
+        walk.is_skip = first_skip;
+        return first_tile;
+    };
+    const auto decay = [&](int hg) {
+        if constexpr ((MOD & kDecay) != 0) score.slope = p.slopes != nullptr ? p.slopes[hk * p.group + hg] * kScoreUnit : 0.f;
+    };
+    if (tile >= 0) {
+        decay(head);
+        int buf = 0, head_of = head;                               // head_of: of the tile in use
         bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
-        __syncthreads();                                           // the tiles of the head before have been read
-        if (tile >= 0) { issue(tile, lds); put(0); }
+        issue(tile, lds);
+        put(0);
         while (tile >= 0) {
             const int i0 = tile * TQ;
             char *lds_q = lds + buf * 2 * kTileBytes, *lds_g = lds_q + kTileBytes;
             const float *lse_of = lds_stat[buf][0], *delta_of = lds_stat[buf][1];
-            const int next = walk.next(look);
+            const int next = advance();
             FD::wait();
             place_id = next_id;
             __syncthreads();
             buf ^= 1;
             if (next >= 0) issue(next, lds + buf * 2 * kTileBytes);
-            if (!whole) {                                          // a bad row of q has a lse of NaN, one of dout a delta
+            if (!whole && __any(!(__builtin_fabsf(delta_of[lane % TQ]) < kInf))) {   // a row that is not finite, hidden from some keys
                 FD::clean_share(lds_q);
                 FD::clean_share(lds_g);
                 __syncthreads();
@@ -346,11 +375,12 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                     seen = seen_from(see);
                 }
                 const float at_row = (float)(i0 + off + 4 * half - key);
+                at_lane.renew();
                 constexpr int kAhead = kAlone<T, DP> ? 4 : 2;         // steps that fragments are read ahead
                 constexpr int N = QB * C, W = N < kAhead ? N : kAhead, F = ST * DB, NF = QB * F, WF = NF < kAhead ? NF : kAhead;
-                frag qf[W], gf[W], gt[WF], qt[WF], pf, sf;
+                frag qf[W], gf[W], gt[WF], qt[WF], pf[QB][ST], sf[QB][ST];    // pf, sf: weights and their gradients, rounded
                 fx16 s[QB], dp[QB];
-                fx4 lse[4], delta[4];
+                fx4 lse[2], delta[2];                              // of four registers' rows, one group ahead
                 const auto read_rows = [&](int n) {
                     qf[n % W] = TL::rows(lds_q, at_lane, 32 * (n / C), n % C);
                     gf[n % W] = TL::rows(lds_g, at_lane, 32 * (n / C), n % C);
@@ -361,8 +391,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                     qt[n % WF] = TL::cols(lds_q, at_lane, row, n % DB);
                 };
                 const auto read_stats = [&](int qb, int g4) {
-                    lse[g4] = *(const fx4 *)(lse_of + 32 * qb + 8 * g4 + 4 * half);
-                    delta[g4] = *(const fx4 *)(delta_of + 32 * qb + 8 * g4 + 4 * half);
+                    lse[g4 & 1] = *(const fx4 *)(lse_of + 32 * qb + 8 * g4 + 4 * half);
+                    delta[g4 & 1] = *(const fx4 *)(delta_of + 32 * qb + 8 * g4 + 4 * half);
                 };
                 const auto scores = [&](int n) {                   // one step of the products behind scores and their gradients
                     const int qb = n / C, c = n % C;
@@ -370,25 +400,38 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                     dp[qb] = AT::mma(gf[n % W], vf[c], c == 0 ? fx16{} : dp[qb]);
                     if (n + W < N) read_rows(n + W);
                 };
-                const auto weight = [&](int qb, int r, bool masked) {
-                    const float li = lse[r >> 2][r & 3], de = delta[r >> 2][r & 3];
-                    float e, g, grad = 1.f;
-                    if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][r], score.unit, -li));
-                    else e = __builtin_amdgcn_exp2f(score(s[qb][r], at_row + (float)(32 * qb + 8 * (r >> 2) + (r & 3)), grad) - li);
-                    g = e * (dp[qb][r] - de);
-                    if constexpr ((MOD & kCap) != 0) g *= grad;
-                    if (masked) {
-                        e = seen.or_zero(__builtin_fmaf(de, 0.f, e), qb, r);
-                        g = seen.or_zero(g, qb, r);
+                // the weights of two registers, rounded at once so that they take a quarter of the registers
+                const auto weights = [&](int qb, int pair, bool masked) {
+                    typedef T two __attribute__((ext_vector_type(2)));
+                    if (pair % 2 == 0 && pair < 6) read_stats(qb, pair / 2 + 1);
+                    float e[2], g[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int r = 2 * pair + k;
+                        const float li = lse[r >> 2 & 1][r & 3], de = delta[r >> 2 & 1][r & 3];
+                        float grad = 1.f;
+                        if constexpr (MOD == kPlain) e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][r], score.unit, -li));
+                        else e[k] = __builtin_amdgcn_exp2f(score(s[qb][r], at_row + (float)(32 * qb + 8 * (r >> 2) + (r & 3)), grad) - li);
+                        g[k] = e[k] * (dp[qb][r] - de);
+                        if constexpr ((MOD & kCap) != 0) g[k] *= grad;
+                        if (masked) {
+                            e[k] = seen.or_zero(__builtin_fmaf(de, 0.f, e[k]), qb, r);
+                            g[k] = seen.or_zero(g[k], qb, r);
+                        }
                     }
-                    s[qb][r] = e;
-                    dp[qb][r] = g;
+                    union { frag f; two t[AT::E / 2]; } u, v;
+                    const int st = 2 * pair / AT::E, at2 = pair % (AT::E / 2);
+                    u.f = pf[qb][st];
+                    v.f = sf[qb][st];
+                    u.t[at2] = two{(T)e[0], (T)e[1]};
+                    v.t[at2] = two{(T)g[0], (T)g[1]};
+                    pf[qb][st] = u.f;
+                    sf[qb][st] = v.f;
                 };
                 const auto gradients = [&](int n) {                // one step of the gradients' products
                     const int qb = n / F, i = n % F;
-                    if (i % DB == 0) { pf = pack<T>(s[qb], i / DB); sf = pack<T>(dp[qb], i / DB); }
-                    dv[i % DB] = AT::mma(gt[n % WF], pf, dv[i % DB]);
-                    dk[i % DB] = AT::mma(qt[n % WF], sf, dk[i % DB]);
+                    dv[i % DB] = AT::mma(gt[n % WF], pf[qb][i / DB], dv[i % DB]);
+                    dk[i % DB] = AT::mma(qt[n % WF], sf[qb][i / DB], dk[i % DB]);
                     if (n + WF < NF) read_cols(n + WF);
                 };
 #pragma unroll
@@ -399,11 +442,10 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                     // between the score products of the second, and theirs between the gradient products of the first.  No
                     // branch may stand between them, so every tile is masked (2 x 4096 positions, 32 heads of 128, causal: the whole
                     // backward pass 1.37 ms with the steps one after the other, 1.23 ms so).
-                    constexpr int EC = (16 + C - 1) / C, EF = (16 + F - 1) / F;
+                    constexpr int EC = (8 + C - 1) / C, EF = (8 + F - 1) / F;   // pairs a step
 #pragma unroll
                     for (int c = 0; c < C; c++) { scores(c); FLK_KEEP_ORDER(); }
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; g4++) read_stats(0, g4);
+                    read_stats(0, 0);
 #pragma unroll
                     for (int c = 0; c < C; c++) {
                         scores(C + c);
@@ -411,17 +453,16 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                         for (int n = c * WF / C; n < (c + 1) * WF / C; n++) read_cols(n);
 #pragma unroll
                         for (int r = c * EC; r < (c + 1) * EC; r++)
-                            if (r < 16) weight(0, r, true);
+                            if (r < 8) weights(0, r, true);
                         FLK_KEEP_ORDER();
                     }
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; g4++) read_stats(1, g4);
+                    read_stats(1, 0);
 #pragma unroll
                     for (int i = 0; i < F; i++) {
                         gradients(i);
 #pragma unroll
                         for (int r = i * EF; r < (i + 1) * EF; r++)
-                            if (r < 16) weight(1, r, true);
+                            if (r < 8) weights(1, r, true);
                         FLK_KEEP_ORDER();
                     }
 #pragma unroll
@@ -436,18 +477,18 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
 #pragma unroll
                             for (int n = 0; n < WF; n++) read_cols(n);
                         }
+                        read_stats(qb, 0);
                         FLK_KEEP_ORDER();
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            if (r % 4 == 0) read_stats(qb, r / 4);
-                            weight(qb, r, masked);
-                        }
+                        for (int r = 0; r < 8; r++) weights(qb, r, masked);
+                        FLK_KEEP_ORDER();
 #pragma unroll
                         for (int i = 0; i < F; i++) { gradients(qb * F + i); FLK_KEEP_ORDER(); }
                     }
                 }
             }
             if (next >= 0) put(buf);
+            if (head != head_of) { head_of = head; decay(head); }
             tile = next;
             whole = walk.is_whole;
             full = walk.is_full;

@@ -53,54 +53,55 @@ template <> struct AttnType<bf16_t> {
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-// Whether any value of 16 bytes is an infinity or a NaN: its exponent bits are all ones.
-template <typename T> __device__ __forceinline__ bool any_nonfinite(ux4 u) {
-    bool bad = false;
+// Whether values are infinities or NaNs: their exponent bits are all ones, and one more in the last of them carries into the
+// sign's place.  Gathered over many chunks by bad_bits, asked once by any_bad.
+template <typename T> __device__ __forceinline__ unsigned bad_bits(ux4 u) {
+    constexpr unsigned m = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16_t>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr unsigned one = m & (0u - m), step = sizeof(T) == 4 ? one : one | one << 16;
+    unsigned r = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) bad |= (u[i] & 0x7f800000u) == 0x7f800000u;
-        else {
-            constexpr unsigned m = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
-            bad |= (u[i] & m) == m || (u[i] >> 16 & m) == m;
-        }
-    }
-    return bad;
+    for (int i = 0; i < 4; i++) r |= (u[i] & m) + step;
+    return r;
 }
+template <typename T> __device__ __forceinline__ bool any_bad(unsigned bits) { return (bits & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u)) != 0; }
+template <typename T> __device__ __forceinline__ bool any_nonfinite(ux4 u) { return any_bad<T>(bad_bits<T>(u)); }
 
-// A tile of rows in LDS, `DP` values each.  Its 16-byte chunks are permuted within a row by an exclusive or with swz(row):
-// eight consecutive rows put the same chunk into different banks (row-wise fragments), and four consecutive rows put
-// the same pair of chunks into different banks (fragments read across the rows).
+// A tile of rows in LDS, `DP` values each.  Its 16-byte chunks are permuted within a row by an exclusive or with swz(row), so that
+// what is read in one cycle, 256 bytes from all 64 banks, lies in different banks: one chunk of 16 rows (row-wise fragments)
+// and four neighbouring chunks of four rows (fragments read across the rows).  Rows of less than 256 bytes begin in
+// different banks already and need fewer bits.  (128 16-bit values a row: 4 and 2 cycles a fragment's instruction where eight
+// permuted rows gave 8 and 4.)  For float, whose matrix instructions take 16 times as long, eight rows are enough.
 template <typename T, int DP> struct Tile {
     static constexpr int RB = DP * (int)sizeof(T), NC = RB / 16;
+    static constexpr int XB = sizeof(T) == 4 ? 3 : RB % 256 == 0 ? 4 : RB % 128 == 0 ? 3 : 2;      // chunk bits that are permuted
+    static constexpr int kPeriod = sizeof(T) == 4 ? 8 : 16;                                        // rows after which it repeats
     static __device__ __forceinline__ int swz(int r) {
-        if constexpr (RB % 128 == 0) return (r & 3) << 1 | (r >> 2 & 1);
-        else return (r & 2) | (r >> 2 & 1);        // rows of 64 or 192 bytes already alternate between two halves of the banks
+        if constexpr (sizeof(T) == 4) return (r & 3) << 1 | (r >> 2 & 1);
+        else if constexpr (XB == 4) return (r & 3) << 2 | (r >> 2 & 3);
+        else if constexpr (XB == 3) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+        else return r >> 2 & 3;
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
 
     typedef typename AttnType<T>::frag frag;
-    // This lane's places in a tile.  Only the low bits of a chunk's number are permuted, so a handful of offsets and
-    // constants on top of them reach every fragment.
-    static constexpr int RV = RB % 128 == 0 ? 4 : 2, CV = sizeof(T) == 4 ? 4 : RB % 128 == 0 ? 2 : 1;
+    // This lane's places in a tile: of chunk `half` of its row, and of its part of a fragment across the first rows.  The bits
+    // that are permuted lie below a row's, so an exclusive or with a constant leads to every other fragment.
+    static constexpr int RV = 1 << (XB - 1), DV = 1 << (XB - 2);
     struct Lane {
-        int r[RV], c[CV];
+        int r, c;
         __device__ __forceinline__ void init() {
             const int l = threadIdx.x & 63, h = l >> 5, m = l & 31;
-#pragma unroll
-            for (int x = 0; x < RV; x++) r[x] = at(m, 2 * x + h);
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int x = 0; x < 4; x++) c[x] = at(4 * h + x, m >> 2) + (m & 3) * 4;
-            } else {
-                // the transposing read: of 16 lanes, four each name 4 values of one row; lane i gets column i of the four rows
-#pragma unroll
-                for (int x = 0; x < CV; x++) c[x] = at(4 * h + (l >> 2 & 3), 4 * x + 2 * (l >> 4 & 1) + (l >> 1 & 1)) + (l & 1) * 8;
-            }
+            r = at(m, h);
+            if constexpr (sizeof(T) == 4) c = at(4 * h, m >> 2) + (m & 3) * 4;
+            // the transposing read: of 16 lanes, four each name 4 values of one row; lane i gets column i of the four rows
+            else c = at(4 * h + (l >> 2 & 3), 2 * (l >> 4 & 1) + (l >> 1 & 1)) + (l & 1) * 8;
         }
+        // keeps the compiler from holding all the derived places in registers for the whole of a loop
+        __device__ __forceinline__ void renew() { asm volatile("" : "+v"(r), "+v"(c)); }
     };
     // step c of the row of this lane (row0 + lane % 32; row0 a multiple of 32)
     static __device__ __forceinline__ frag rows(const char *tile, const Lane &p, int row0, int c) {
-        return *(const frag *)(tile + p.r[c % RV] + row0 * RB + c / RV * RV * 32);
+        return *(const frag *)(tile + (p.r ^ (c % RV * 32)) + row0 * RB + c / RV * RV * 32);
     }
     // columns 32 db + lane % 32 of KS rows from row0 on (a multiple of KS), in the order in which the accumulator registers
     // hold rows
@@ -108,13 +109,13 @@ template <typename T, int DP> struct Tile {
         frag f;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) f[i] = *(const float *)(tile + p.c[i] + row0 * RB + db * 128);
+            for (int i = 0; i < 4; i++) f[i] = *(const float *)(tile + (p.c ^ (i * 32)) + (row0 + i) * RB + db * 128);
         } else {
             union { sx4 s[2]; frag f; } u;
 #pragma unroll
             for (int k = 0; k < 2; k++)
-                u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) sx4 *)(tile + p.c[db % CV] + (row0 + 8 * k) * RB + db / CV * CV * 64));
+                u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4 *)(
+                    tile + (p.c ^ (db % DV * 64 + k * 32)) + (row0 + 8 * k) * RB + db / DV * DV * 64));
             f = u.f;
         }
         return f;
@@ -134,7 +135,6 @@ template <typename T> __device__ __forceinline__ typename AttnType<T>::frag pack
 
 // Infinities and NaNs of a tile must not reach rows that hide them, but a product with weight zero would carry them there.
 // They are set to zero in LDS where a mask is needed; clean() does it to this thread's 16 bytes.
-template <typename T> __device__ __forceinline__ bool any_nonfinite(ux4 u);
 template <typename T> __device__ __forceinline__ void clean(char *at) {
     union { ux4 u; T t[16 / sizeof(T)]; } x;
     x.u = *(const ux4 *)at;
@@ -215,7 +215,7 @@ template <typename T, int DP, int TR> struct Feed {
     typedef Tile<T, DP> TL;
     static constexpr int NC = TL::NC, N = TR * NC / kAttnThreads, kStep = kAttnThreads / NC;
     static_assert(TR * NC % kAttnThreads == 0, "every instruction is full");
-    static constexpr bool kEven = kAttnThreads % NC == 0 && kStep % 8 == 0;   // all instructions permute alike
+    static constexpr bool kEven = kAttnThreads % NC == 0 && kStep % TL::kPeriod == 0;   // all instructions permute alike
     const T *base;
     int64_t stride;
     unsigned off[kEven ? 1 : N];
@@ -263,10 +263,10 @@ template <typename T, int DP, int TR> struct Feed {
     }
     // whether this thread's share of a tile in LDS holds an infinity or a NaN
     static __device__ __forceinline__ bool nonfinite(const char *tile) {
-        bool bad = false;
+        unsigned bits = 0;
 #pragma unroll
-        for (int n = 0; n < N; n++) bad |= any_nonfinite<T>(*(const ux4 *)(tile + (n * kAttnThreads + threadIdx.x) * 16));
-        return bad;
+        for (int n = 0; n < N; n++) bits |= bad_bits<T>(*(const ux4 *)(tile + (n * kAttnThreads + threadIdx.x) * 16));
+        return any_bad<T>(bits);
     }
 };
 

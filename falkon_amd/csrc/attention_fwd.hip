@@ -12,7 +12,7 @@ namespace flk {
 constexpr float kSlack = 6.f;
 
 template <typename T, int DP, int MOD>
-__global__ void __launch_bounds__(kAttnThreads, 2) attention_fwd_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) attention_fwd_kernel(AttnArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
