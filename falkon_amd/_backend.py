@@ -81,10 +81,10 @@ _BSH = [c_void_p, c_int64, c_int64, c_int64]        # ptr, strides of batch, row
 _ATTN_SIZES = [c_int64] * 7                         # batch, queries, keys, heads, key heads, d, dv
 _ATTN_SCORE = [ctypes.c_double, ctypes.c_double, c_void_p]
 _SIGNATURES["flk_attention_max_d"] = (c_int64, [c_int])
-_SIGNATURES["flk_attention_workspace_bytes"] = (c_size_t, [c_int64, c_int64, c_int])
+_SIGNATURES["flk_attention_workspace_bytes"] = (c_size_t, [c_int64] * 5 + [c_int, c_int])
 _SIGNATURES["flk_attention"] = (c_int, [*_BSH, *_BSH, *_BSH, *_ATTN_SIZES, *_ATTN_SCORE, c_int, c_void_p, c_void_p, c_int64,
                                         c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p])
-_SIGNATURES["flk_attention_backward_workspace_bytes"] = (c_size_t, [*_ATTN_SIZES, c_int, c_int])
+_SIGNATURES["flk_attention_backward_workspace_bytes"] = (c_size_t, [*_ATTN_SIZES, c_int, c_int, c_int])
 _SIGNATURES["flk_attention_backward"] = (c_int, [*_BSH, *_BSH, *_BSH, c_void_p, c_void_p, c_void_p, *_BSH, *_ATTN_SIZES, *_ATTN_SCORE, c_int,
                                                  c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                                  c_void_p, c_size_t, c_void_p])

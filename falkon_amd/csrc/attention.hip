@@ -34,13 +34,43 @@ __global__ void __launch_bounds__(kAttnThreads) attention_dslopes_kernel(const f
     if (threadIdx.x == 0) out[blockIdx.x] = (float)lds[0];
 }
 
-// dk or dv from its parts
-template <typename T>
-__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(const float *part, int64_t n, int parts, T *out) {
-    for (int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kAttnThreads) {
-        float s = 0.f;
-        for (int k = 0; k < parts; k++) s += part[k * n + i];
-        out[i] = (T)s;
+// out, rest and lse from the parts of the forward kernel, one thread a value
+template <typename T> __global__ void __launch_bounds__(kAttnThreads) attention_parts_kernel(AttnArgs p) {
+    const int64_t rows = (int64_t)p.b * p.sq * p.hq, i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x;
+    if (i >= rows * p.dv_d) return;
+    const int64_t row = i / p.dv_d, c = i % p.dv_d;
+    float top = -kInf;
+    for (int k = 0; k < p.parts; k++) top = fmaxf(top, p.part_ml[(k * rows + row) * 2]);
+    float x = 0.f, l = 0.f;
+    for (int k = 0; k < p.parts; k++) {
+        const float m = p.part_ml[(k * rows + row) * 2], lk = p.part_ml[(k * rows + row) * 2 + 1];
+        if (m == -kInf && lk == 0.f) continue;                     // saw nothing
+        const float a = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        x += a * p.part_o[(k * rows + row) * p.dv_d + c];
+        l += a * lk;
+    }
+    const float y = l == 0.f ? 0.f : x / l;
+    const T z = (T)y;
+    ((T *)p.o)[i] = z;
+    if (p.rest != nullptr) ((T *)p.rest)[i] = (T)(y - (float)z);
+    if (c == 0 && p.lse != nullptr) {
+        const int64_t h = row % p.hq, s = row / p.hq % p.sq, b = row / p.hq / p.sq;
+        p.lse[(b * p.hq + h) * p.sq + s] = l == 0.f ? -kInf : top * kLn2 + __logf(l);
+    }
+}
+
+// dq, dk and dv from their parts
+struct JoinArgs { const float *part[3]; void *to[3]; int64_t n[3]; int parts[3]; };
+template <typename T> __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(JoinArgs p) {
+    int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        if (i >= 0 && i < p.n[k]) {
+            float s = 0.f;
+            for (int j = 0; j < p.parts[k]; j++) s += p.part[k][j * p.n[k] + i];
+            ((T *)p.to[k])[i] = (T)s;
+        }
+        i -= p.n[k];
     }
 }
 
@@ -68,21 +98,39 @@ static void place_docs(AttnArgs &a, void *ws) {
     a.doc_ids = (int *)((char *)ws + align256((size_t)a.b * a.doc_blocks * sizeof(int2)));
 }
 
-struct AttnSizes { int64_t doc_blocks, docs, sq_pad, stats, slopes, parts; int splits; };
-static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, bool docs, bool slopes) {
+// Workgroups among which a tile of 128 rows divides its tiles of keys (or queries).  One wave's way through them all takes its
+// time however few workgroups there are, so where they do not fill the chip they are made shorter: up to 512 in all, none
+// with less than eight tiles (four of float, which take four times as long).  The parts are written in float and read again,
+// so there are no more than eight.
+// (Float, 2 x 8 heads of 80, 1000 positions: forward 116 -> 78 us, backward 379 -> 222; bf16, 8 heads of 128, 2048 positions:
+// forward 53 -> 50, backward 161 -> 129.)
+static int parts_for(int64_t groups, int64_t keys, int dtype) {
+    const int64_t most = elem_size(dtype) == 4 ? cdiv(keys, 32) / 4 : cdiv(keys, 64) / 8;
+    int64_t n = groups > 0 ? 512 / groups : 1;
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+
+struct AttnSizes { int64_t doc_blocks, docs, sq_pad, stats, slopes, dq, dkv; int parts, head_parts, row_parts; };
+static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, bool docs, bool slopes, int dtype) {
     AttnSizes z = {};
     z.doc_blocks = cdiv(sk, kDocBlock);
     z.docs = docs ? doc_bytes(b, sk) : 0;
     z.sq_pad = cdiv(sq, kAttnRows) * kAttnRows;
     z.stats = align256((size_t)(b * hq * z.sq_pad) * 8);
     z.slopes = slopes ? align256((size_t)(b * hq * cdiv(sq, kAttnRows)) * 4) : 0;
-    // The dk / dv kernel has one workgroup for 128 keys of a key head; where that leaves compute units idle, the query heads
-    // that share the key head are divided over several, whose parts are added afterwards.
+    // (the slopes' gradient is a product of two of a row's sums, so their rows are not divided)
+    z.parts = slopes ? 1 : parts_for(b * hq * cdiv(sq, kAttnRows), sk, dtype);
+    z.dq = z.parts > 1 ? align256((size_t)z.parts * b * sq * hq * d * 4) : 0;
+    // dk / dv: the query heads that share the key head are divided first, then the tiles of queries
     const int64_t groups = b * hk * cdiv(sk, kAttnRows), group = hk > 0 ? hq / hk : 1;
-    z.splits = 1;
-    if (groups > 0 && groups < 512) z.splits = (int)(cdiv(512, groups) < group ? cdiv(512, groups) : group);
-    if (z.splits < 1) z.splits = 1;
-    z.parts = z.splits > 1 ? align256((size_t)z.splits * b * sk * hk * (d + dv) * 4) : 0;
+    z.head_parts = 1;
+    if (groups > 0 && groups < 512) z.head_parts = (int)(cdiv(512, groups) < group ? cdiv(512, groups) : group);
+    if (z.head_parts < 1) z.head_parts = 1;
+    if (z.head_parts > 8) z.head_parts = 8;
+    z.row_parts = parts_for(groups * z.head_parts, sq, dtype);
+    if (z.row_parts * z.head_parts > 8) z.row_parts = 8 / z.head_parts;
+    z.dkv = z.head_parts * z.row_parts > 1 ? align256((size_t)z.head_parts * z.row_parts * b * sk * hk * (d + dv) * 4) : 0;
     return z;
 }
 
@@ -118,14 +166,46 @@ template <typename T> static int attention_backward_impl(AttnArgs &a, int dp, fl
                            (int64_t)a.b * cdiv(a.sq, kAttnRows), dslopes);
         FLK_LAUNCH_CHECK("attention_dslopes_kernel");
     }
-    if (a.dk == nullptr || (int64_t)a.b * a.sk == 0) return FLK_OK;
-    if ((rc = launch_attention_dkv<T>(a, dp, st)) != FLK_OK || a.splits == 1) return rc;
-    const int64_t nk = (int64_t)a.b * a.sk * a.hk * a.d, nv = (int64_t)a.b * a.sk * a.hk * a.dv_d;
-    const auto grid = [](int64_t n) { return dim3((unsigned)(cdiv(n, kAttnThreads) < 4096 ? cdiv(n, kAttnThreads) : 4096)); };
-    hipLaunchKernelGGL((attention_join_kernel<T>), grid(nk), dim3(kAttnThreads), 0, st, a.dkv_part, nk, a.splits, (T *)a.dk);
-    hipLaunchKernelGGL((attention_join_kernel<T>), grid(nv), dim3(kAttnThreads), 0, st, a.dkv_part + a.splits * nk, nv, a.splits, (T *)a.dv);
+    JoinArgs join = {};
+    if (a.dq != nullptr && a.parts > 1) {
+        join.part[0] = a.dq_part; join.to[0] = a.dq; join.n[0] = (int64_t)a.b * a.sq * a.hq * a.d; join.parts[0] = a.parts;
+    }
+    if (a.dk != nullptr && (int64_t)a.b * a.sk > 0) {
+        if ((rc = launch_attention_dkv<T>(a, dp, st)) != FLK_OK) return rc;
+        const int splits = a.head_parts * a.row_parts;
+        if (splits > 1) {
+            const int64_t keys = (int64_t)a.b * a.sk * a.hk, nk = keys * a.d;
+            join.part[1] = a.dkv_part; join.to[1] = a.dk; join.n[1] = nk; join.parts[1] = splits;
+            join.part[2] = a.dkv_part + splits * nk; join.to[2] = a.dv; join.n[2] = keys * a.dv_d; join.parts[2] = splits;
+        }
+    }
+    const int64_t n = join.n[0] + join.n[1] + join.n[2];
+    if (n == 0) return FLK_OK;
+    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)cdiv(n, kAttnThreads)), dim3(kAttnThreads), 0, st, join);
     FLK_LAUNCH_CHECK("attention_join_kernel");
     return FLK_OK;
+}
+
+template <typename T> static int attention_forward_impl(AttnArgs &a, int dp, hipStream_t st) {
+    const int rc = launch_attention_fwd<T>(a, dp, st);
+    if (rc != FLK_OK || a.parts == 1) return rc;
+    const int64_t n = (int64_t)a.b * a.sq * a.hq * a.dv_d;
+    hipLaunchKernelGGL((attention_parts_kernel<T>), dim3((unsigned)cdiv(n, kAttnThreads)), dim3(kAttnThreads), 0, st, a);
+    FLK_LAUNCH_CHECK("attention_parts_kernel");
+    return FLK_OK;
+}
+
+// forward: the documents' spans and ids, then the parts of out and of the rows' maxima and sums
+struct FwdSizes { int64_t docs, o, ml; int parts; };
+static FwdSizes fwd_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t dv, bool docs, int dtype) {
+    FwdSizes z = {};
+    z.docs = docs ? doc_bytes(b, sk) : 0;
+    z.parts = parts_for(b * hq * cdiv(sq, kAttnRows), sk, dtype);
+    if (z.parts > 1) {
+        z.o = align256((size_t)z.parts * b * sq * hq * dv * 4);
+        z.ml = align256((size_t)z.parts * b * sq * hq * 8);
+    }
+    return z;
 }
 
 // Workgroups the keys of a sequence are divided over, none of them with less than four tiles a wave at the cache's capacity.
@@ -151,9 +231,10 @@ extern "C" {
 
 int64_t flk_attention_max_d(int dtype) { return attn_dtype(dtype) ? kAttnMaxD : 0; }
 
-size_t flk_attention_workspace_bytes(int64_t b, int64_t sk, int with_documents) {
-    if (b < 0 || sk < 0 || sk > kMaxPositions || !with_documents) return 0;
-    return (size_t)doc_bytes(b, sk);
+size_t flk_attention_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t dv, int with_documents, int dtype) {
+    if (b < 0 || sq < 0 || sk < 0 || sq > kMaxPositions || sk > kMaxPositions || hq < 1 || dv < 1 || !attn_dtype(dtype)) return 0;
+    const FwdSizes z = fwd_sizes(b, sq, sk, hq, dv, with_documents != 0, dtype);
+    return (size_t)(z.docs + z.o + z.ml);
 }
 
 int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
@@ -165,7 +246,8 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
     int rc = attn_check("flk_attention", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
     if (rc != FLK_OK || b * sq == 0) return rc;
     if (q == nullptr || out == nullptr || (sk > 0 && (k == nullptr || v == nullptr))) return fail(FLK_EINVAL, "flk_attention: null pointer");
-    const size_t need = flk_attention_workspace_bytes(b, sk, documents != nullptr);
+    const FwdSizes z = fwd_sizes(b, sq, sk, hq, dv, documents != nullptr, dtype);
+    const size_t need = (size_t)(z.docs + z.o + z.ml);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     AttnArgs a = {};
@@ -174,22 +256,27 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
     a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
     a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
     a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)cdiv(sk, kDocBlock);
-    place_docs(a, workspace);
+    a.parts = z.parts;
+    char *ws = (char *)workspace;
+    place_docs(a, ws); ws += z.docs;
+    a.part_o = (float *)ws; ws += z.o;
+    a.part_ml = (float *)ws;
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) && aligned16(out) && aligned16(a.rest);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);
-#define FLK_CALL(T) launch_attention_fwd<T>(a, dp, st)
+#define FLK_CALL(T) attention_forward_impl<T>(a, dp, st)
     return FLK_BY_TYPE(dtype, FLK_CALL);
 #undef FLK_CALL
 }
 
 size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
-                                              int with_slopes, int with_documents) {
-    if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1 || hq % hk != 0 || sq > kMaxPositions || sk > kMaxPositions) return 0;
-    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, with_documents != 0, with_slopes != 0);
-    return (size_t)(z.docs + z.stats + z.slopes + z.parts);
+                                              int with_slopes, int with_documents, int dtype) {
+    if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1 || hq % hk != 0 || sq > kMaxPositions || sk > kMaxPositions || !attn_dtype(dtype))
+        return 0;
+    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, with_documents != 0, with_slopes != 0, dtype);
+    return (size_t)(z.docs + z.stats + z.slopes + z.dq + z.dkv);
 }
 
 int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
@@ -205,8 +292,8 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     if (dslopes != nullptr && slopes == nullptr) return fail(FLK_EINVAL, "flk_attention_backward: no slopes to differentiate");
     if ((b * sq > 0 && (q == nullptr || out == nullptr || lse == nullptr || dout == nullptr)) || (b * sk > 0 && (k == nullptr || v == nullptr)))
         return fail(FLK_EINVAL, "flk_attention_backward: null pointer");
-    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, documents != nullptr, dslopes != nullptr);
-    const size_t need = (size_t)(z.docs + z.stats + z.slopes + z.parts);
+    const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, documents != nullptr, dslopes != nullptr, dtype);
+    const size_t need = (size_t)(z.docs + z.stats + z.slopes + z.dq + z.dkv);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     AttnArgs a = {};
@@ -215,11 +302,13 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     a.dos = {do_b, do_s, do_h}; a.sq_pad = z.sq_pad;
     a.b = (int)b; a.sq = (int)sq; a.sk = (int)sk; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d; a.dv_d = (int)dv;
     a.scale = (float)scale; a.cap = (float)softcap; a.slopes = slopes; a.causal = causal != 0; a.prefix = prefix;
-    a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)z.doc_blocks; a.splits = z.splits;
+    a.docs = documents; a.docs_b = documents_b; a.doc_blocks = (int)z.doc_blocks;
+    a.parts = z.parts; a.head_parts = z.head_parts; a.row_parts = z.row_parts;
     char *ws = (char *)workspace;
     place_docs(a, ws); ws += z.docs;
     a.stats = (float *)ws; ws += z.stats;
     a.dslopes_part = dslopes != nullptr ? (float *)ws : nullptr; ws += z.slopes;
+    a.dq_part = (float *)ws; ws += z.dq;
     a.dkv_part = (float *)ws;
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) &&

@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int heads = p.b * p.hq, pairs = p.b * p.hk;
     const int hb = blockIdx.x % heads, tiles_q = (p.sq + kAttnRows - 1) / kAttnRows;
-    const int tile_q = tiles_q - 1 - blockIdx.x / heads;
+    const int tile_q = tiles_q - 1 - blockIdx.x / heads % tiles_q, part = blockIdx.x / heads / tiles_q;
     const int b = hb % pairs / p.hk, hk = hb % p.hk, h = hk * p.group + hb / pairs;
     const int off = p.sk - p.sq;
     const int i0 = tile_q * kAttnRows, row = i0 + wave * 32 + (lane & 31);
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         const float x = p.lse[((int64_t)b * p.hq + h) * p.sq + row];
         lse = x == -kInf ? kInf : x * kScoreUnit;
     }
-    if (half == 0) {
+    if (half == 0 && part == 0) {
         float *st = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad + row;
         st[0] = lse;
         st[p.sq_pad] = delta;
@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     }
     const int key_end = p.causal ? max(min(pos_end, p.sk), prefix) : p.sk;
     TileWalk walk;
-    walk.start(0, key_end > 0 ? (key_end + TK - 1) / TK : 0);
+    const int64_t tiles_k = key_end > 0 ? (key_end + TK - 1) / TK : 0;
+    walk.start((int)(tiles_k * part / p.parts), (int)(tiles_k * (part + 1) / p.parts));
     const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
         const int k0 = t * TK, k1 = k0 + TK;
         const bool inside = k1 <= p.sk, in_prefix = !p.causal || k1 <= prefix;
@@ -222,8 +223,12 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     if (p.dq == nullptr) return;
     __syncthreads();
     const float unscale = p.scale * score.kGrad;
-    store_rows<T, DP>(lds + wave * 32 * TL::RB, [&](int db, int r) { return acc[db][r] * unscale; },
-                      (T *)p.dq + (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, (int64_t)p.hq * p.d, p.sq - (i0 + wave * 32), p.d, p.vec);
+    const int64_t to = (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, row_q = (int64_t)p.hq * p.d;
+    const auto value = [&](int db, int r) { return acc[db][r] * unscale; };
+    const int rows = p.sq - (i0 + wave * 32);
+    if (p.parts == 1) store_rows<T, DP>(lds + wave * 32 * TL::RB, value, (T *)p.dq + to, row_q, rows, p.d, p.vec);
+    else                                                           // parts in float, added by attention_join_kernel
+        store_rows<float, DP>(lds + wave * 32 * Tile<float, DP>::RB, value, p.dq_part + part * (int64_t)p.b * p.sq * row_q + to, row_q, rows, p.d, p.d % 4 == 0);
 }
 
 // Whether the dk / dv kernel's fragments and sums (keys, values, dk and dv of 32 keys in registers) leave room for one wave a SIMD only
@@ -243,7 +248,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int pairs = p.b * p.hk, tiles_k = (p.sk + kAttnRows - 1) / kAttnRows;
-    const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs % p.splits, tile_k = blockIdx.x / pairs / p.splits;
+    const int splits = p.head_parts * p.row_parts, pair = blockIdx.x % pairs, split = blockIdx.x / pairs % splits;
+    const int tile_k = blockIdx.x / pairs / splits, head_part = split % p.head_parts, row_part = split / p.head_parts;
     const int b = pair / p.hk, hk = pair % p.hk;
     const int off = p.sk - p.sq;
     const int k0 = tile_k * kAttnRows, k_lo = k0 + wave * 32, key = k_lo + (lane & 31);
@@ -299,8 +305,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
 
     // the heads that share this key head, one after the other; the tiles to visit are the same for each
-    int head = p.group * split / p.splits;                         // of the tile on its way
-    const int head_end = p.group * (split + 1) / p.splits;
+    int head = p.group * head_part / p.head_parts;                 // of the tile on its way
+    const int head_end = p.group * (head_part + 1) / p.head_parts;
     Score<T, MOD> score(p.scale, p.cap, 0.f);
     FD feed_q, feed_g;
     feed_q.init((const T *)p.q + b * p.qs.b + (hk * p.group + head) * p.qs.h, p.qs.s, p.d, p.vec);
@@ -325,7 +331,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     };
     const int tile_lo = lo / TQ, tile_end = (p.sq + TQ - 1) / TQ;
     TileWalk walk, again;
-    walk.start(tile_lo, tile_end);
+    const int64_t tiles_q = max(0, tile_end - tile_lo);
+    walk.start(tile_lo + (int)(tiles_q * row_part / p.row_parts), tile_lo + (int)(tiles_q * (row_part + 1) / p.row_parts));
     int tile = walk.next(look);
     again = walk;                                                  // the first 64 tiles as they were found
     const int first_tile = tile;
@@ -500,7 +507,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int rows = p.sk - k_lo;
     const int64_t line = (int64_t)b * p.sk + k_lo, at_k = (line * p.hk + hk) * p.d, at_v = (line * p.hk + hk) * p.dv_d;
     const int64_t row_k = (int64_t)p.hk * p.d, row_v = (int64_t)p.hk * p.dv_d;
-    if (p.splits == 1) {
+    if (splits == 1) {
         char *mine = lds + wave * 32 * TL::RB;
         store_rows<T, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, (T *)p.dk + at_k, row_k, rows, p.d, p.vec);
         store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r]; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec);
@@ -508,18 +515,18 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
         const int64_t nk = (int64_t)p.b * p.sk * row_k, nv = (int64_t)p.b * p.sk * row_v;
         char *mine = lds + wave * 32 * Tile<float, DP>::RB;
         store_rows<float, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, p.dkv_part + split * nk + at_k, row_k, rows, p.d, p.d % 4 == 0);
-        store_rows<float, DP>(mine, [&](int db, int r) { return dv[db][r]; }, p.dkv_part + p.splits * nk + split * nv + at_v, row_v, rows, p.dv_d,
+        store_rows<float, DP>(mine, [&](int db, int r) { return dv[db][r]; }, p.dkv_part + splits * nk + split * nv + at_v, row_v, rows, p.dv_d,
                               p.d % 4 == 0 && p.dv_d % 4 == 0);
     }
 }
 
 template <typename T> int launch_attention_dq(const AttnArgs &a, int dp, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows)));
+    const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows) * a.parts));
     FLK_ATTN_LAUNCH(attention_dq_kernel, grid)
     return FLK_OK;
 }
 template <typename T> int launch_attention_dkv(const AttnArgs &a, int dp, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.splits * ((a.sk + kAttnRows - 1) / kAttnRows)));
+    const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.head_parts * a.row_parts * ((a.sk + kAttnRows - 1) / kAttnRows)));
     FLK_ATTN_LAUNCH(attention_dkv_kernel, grid)
     return FLK_OK;
 }

@@ -171,12 +171,15 @@ struct AttnStride { int64_t b, s, h; };
 struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
     void *o, *rest, *dq, *dk, *dv;                     // rest: what rounding took from out, for the backward pass
-    float *lse, *dslopes_part, *dkv_part;
+    float *lse, *dslopes_part, *dq_part, *dkv_part;
     float *stats;                                      // backward: [b][hq][2][sq_pad], the rows' lse (in units of log 2) and delta
     int64_t sq_pad;
     AttnStride qs, ks, vs, dos;                        // strides of q, k, v and dout; the others are contiguous
     int b, sq, sk, hq, hk, group, d, dv_d;
-    int splits;                                        // dk / dv: parts the heads of a group are divided into
+    // Workgroups that share a tile's rows, each with a part of its tiles of keys (forward, dq): parts; dk / dv: head_parts, each with
+    // a part of the heads of the group, times row_parts, each with a part of the tiles of queries
+    int parts, head_parts, row_parts;
+    float *part_o, *part_ml;                           // forward: [part][b][sq][hq][dv] and [part][b][sq][hq][2], maximum and sum
     float scale, cap;
     const float *slopes;
     const int *prefix, *docs;

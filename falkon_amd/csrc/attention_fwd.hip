@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     // consecutive workgroups go to different XCDs: heads that share keys stay on one of them, the longest rows go first
     const int heads = p.b * p.hq, pairs = p.b * p.hk;
     const int hb = blockIdx.x % heads, tiles_q = (p.sq + kAttnRows - 1) / kAttnRows;
-    const int tile_q = tiles_q - 1 - blockIdx.x / heads;
+    const int tile_q = tiles_q - 1 - blockIdx.x / heads % tiles_q, part = blockIdx.x / heads / tiles_q;
     const int b = hb % pairs / p.hk, hk = hb % p.hk, h = hk * p.group + hb / pairs;
     const int off = p.sk - p.sq;
     const int i0 = tile_q * kAttnRows, row = i0 + wave * 32 + (lane & 31);
@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     }
     const int key_end = p.causal ? max(min(pos_end, p.sk), prefix) : p.sk;
     TileWalk walk;
-    walk.start(0, key_end > 0 ? (key_end + TK - 1) / TK : 0);
+    const int64_t tiles_k = key_end > 0 ? (key_end + TK - 1) / TK : 0;
+    walk.start((int)(tiles_k * part / p.parts), (int)(tiles_k * (part + 1) / p.parts));
     const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
         const int k0 = t * TK, k1 = k0 + TK;
         const bool inside = k1 <= p.sk, in_prefix = !p.causal || k1 <= prefix;
@@ -235,6 +236,18 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         skip = walk.is_skip;
     }
     l += other_half(l);
+    if (p.parts > 1) {                                             // joined by attention_parts_kernel
+        const int64_t rows_all = (int64_t)p.b * p.sq * p.hq, first = ((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h;
+        __syncthreads();
+        store_rows<float, DP>(lds + wave * 32 * Tile<float, DP>::RB, [&](int db, int r) { return o[db][r]; },
+                              p.part_o + (part * rows_all + first) * p.dv_d, (int64_t)p.hq * p.dv_d, p.sq - (i0 + wave * 32), p.dv_d, p.dv_d % 4 == 0);
+        if (live && half == 0) {
+            float *ml = p.part_ml + (part * rows_all + first + (int64_t)lane * p.hq) * 2;
+            ml[0] = m;
+            ml[1] = l;
+        }
+        return;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;                    // a row that sees nothing is zero
 #pragma unroll
     for (int db = 0; db < DB; db++) o[db] *= inv;
@@ -251,7 +264,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
 }
 
 template <typename T> int launch_attention_fwd(const AttnArgs &a, int dp, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows)));
+    const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows) * a.parts));
     FLK_ATTN_LAUNCH(attention_fwd_kernel, grid)
     return FLK_OK;
 }

@@ -106,12 +106,13 @@ def _forward(q, k, v, slopes, scale, softcap, causal, prefix, documents, want_ls
     # what rounding takes from 16-bit results: dout.out, which the backward pass subtracts from every term, needs it
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     lse = torch.empty((b, hq, sq), dtype=torch.float32, device=q.device) if want_lse else None
-    nbytes = lib.flk_attention_workspace_bytes(b, sk, 1) if documents is not None else 0
+    code = _DTYPE_CODE[q.dtype]
+    nbytes = lib.flk_attention_workspace_bytes(b, sq, sk, hq, dv, documents is not None, code)
     ws = _workspace(nbytes, q.device)
     with _current(q.device):
         rc = lib.flk_attention(*_bsh(q), *_bsh(k), *_bsh(v), b, sq, sk, hq, hk, d, dv, scale, softcap, _ptr(slopes), causal,
                                _ptr(prefix), _ptr(documents), documents.stride(0) if documents is not None else 0,
-                               out.data_ptr(), _ptr(rest), _ptr(lse), _DTYPE_CODE[q.dtype], _ptr(ws), nbytes, _stream_handle(q.device))
+                               out.data_ptr(), _ptr(rest), _ptr(lse), code, _ptr(ws), nbytes, _stream_handle(q.device))
     _backend.raise_for_status(rc, "flk_attention")
     return out, rest, lse
 
@@ -142,13 +143,14 @@ class _AttentionFn(torch.autograd.Function):
             dk, dv_ = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(v.shape, dtype=q.dtype, device=dev)
         if need_slopes:
             dslopes = torch.empty(slopes.shape, dtype=torch.float32, device=dev)
-        nbytes = lib.flk_attention_backward_workspace_bytes(b, sq, sk, hq, hk, d, dv, need_slopes, documents is not None)
+        code = _DTYPE_CODE[q.dtype]
+        nbytes = lib.flk_attention_backward_workspace_bytes(b, sq, sk, hq, hk, d, dv, need_slopes, documents is not None, code)
         ws = _workspace(nbytes, dev)
         with _current(dev):
             rc = lib.flk_attention_backward(
                 *_bsh(q), *_bsh(k), *_bsh(v), out.data_ptr(), _ptr(rest), lse.data_ptr(), *_bsh(dout), b, sq, sk, hq, hk, d, dv, scale, softcap,
                 _ptr(slopes), causal, _ptr(prefix), _ptr(documents), documents.stride(0) if documents is not None else 0,
-                _ptr(dq), _ptr(dk), _ptr(dv_), _ptr(dslopes), _DTYPE_CODE[q.dtype], _ptr(ws), nbytes, _stream_handle(dev))
+                _ptr(dq), _ptr(dk), _ptr(dv_), _ptr(dslopes), code, _ptr(ws), nbytes, _stream_handle(dev))
         _backend.raise_for_status(rc, "flk_attention_backward")
         return dq, dk if need_k else None, dv_ if need_v else None, dslopes, None, None, None, None, None
 

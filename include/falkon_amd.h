@@ -326,7 +326,7 @@ int flk_layer_norm_backward(const void *x, int64_t rows, int64_t d, int64_t x_rs
  * neither) and dslopes (hq floats); each may be NULL.  Sums are made in a fixed order: the same run to run. */
 int64_t flk_attention_max_d(int dtype);
 
-size_t flk_attention_workspace_bytes(int64_t b, int64_t sk, int with_documents);
+size_t flk_attention_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t dv, int with_documents, int dtype);
 
 int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
                   const void *v, int64_t v_b, int64_t v_s, int64_t v_h,
@@ -336,7 +336,7 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
                   void *workspace, size_t workspace_bytes, void *stream);
 
 size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv,
-                                              int with_dslopes, int with_documents);
+                                              int with_dslopes, int with_documents, int dtype);
 
 int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
                            const void *v, int64_t v_b, int64_t v_s, int64_t v_h, const void *out, const void *rest, const float *lse,

@@ -57,6 +57,43 @@ def test_values_and_gradients(size, dtype, causal):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["plain", "causal cap", "prefix", "documents", "decay"])
+@pytest.mark.parametrize("sq,sk,d", [(100, 1500, 64), (700, 1100, 128), (1000, 1000, 50)])
+def test_divided_keys(dtype, kind, sq, sk, d):
+    """Few heads and many keys: a tile's keys, and the queries of a tile of keys, are divided over workgroups."""
+    q, k, v, do = _make(1, sq, sk, 2, 1, d, d, dtype, seed=21)
+    kw = dict(causal=kind not in ("plain", "decay"))
+    if "cap" in kind:
+        kw["softcap"] = 4.0
+    if kind == "prefix":
+        kw["prefix"] = torch.tensor([170], device=DEV)
+    if kind == "documents":
+        kw["documents"] = _ids("long", 1, sk)
+        kw["documents"][:, :200] = -1
+    _check(q, k, v, do, torch.tensor([0.01, 0.2], device=DEV) if kind == "decay" else None, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["plain", "causal cap", "prefix decay", "documents", "documents cap decay"])
+@pytest.mark.parametrize("d", [28, 64, 81, 128])
+def test_many_workgroups(dtype, kind, d):
+    """Enough heads to fill the chip: no tile's keys are divided over workgroups, which the sizes above may be."""
+    b, s, hq, hk = 16, 135, 16, 8
+    q, k, v, do = _make(b, s, s, hq, hk, d, d, dtype, seed=20)
+    kw = dict(causal=kind != "plain")
+    if "cap" in kind:
+        kw["softcap"] = 4.0
+    if "prefix" in kind:
+        kw["prefix"] = torch.arange(b, device=DEV) * 9
+    if "documents" in kind:
+        kw["documents"] = _ids("sorted", b, s)
+    slopes = torch.arange(hq, device=DEV).float() / 40 if "decay" in kind else None
+    _check(q, k, v, do, slopes, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("cap,slope", [(0.0, True), (2.0, False), (30.0, True)])
 @pytest.mark.parametrize("d", [16, 64, 72, 128])
@@ -448,8 +485,9 @@ def test_c_entry_refusals():
         assert call(**bad) == _backend.FLK_EINVAL and _backend.last_error(), bad
     for bad in (dict(d=129), dict(dv=129), dict(sk=(1 << 28) + 1), dict(b=1 << 40), dict(b=1 << 20, sq=1 << 28)):
         assert call(**bad) == _backend.FLK_EUNSUPPORTED, bad
-    need = lib.flk_attention_workspace_bytes(1, 7, 1)
-    assert need > 0 and lib.flk_attention_workspace_bytes(1, 7, 0) == 0
+    need = lib.flk_attention_workspace_bytes(1, 5, 7, 4, 8, 1, 0)
+    assert need > 0 and lib.flk_attention_workspace_bytes(1, 5, 7, 4, 8, 0, 0) == 0
+    assert lib.flk_attention_workspace_bytes(1, 5, 7, 4, 8, 1, 1) == 0
     assert call(docs=one, ws=one, wsb=need - 1) == _backend.FLK_ENOMEM and call(docs=one, wsb=need) == _backend.FLK_ENOMEM
     bnames = ("q qb qs qh k kb ks kh v vb vs vh out rest lse do dob dos doh b sq sk hq hk d dv scale cap slopes causal prefix docs docs_b "
               "dq dk dvo dsl dt ws wsb st").split()
@@ -457,9 +495,9 @@ def test_c_entry_refusals():
     back = lambda **kw: lib.flk_attention_backward(*[{**bbase, **kw}[n] for n in bnames])  # noqa: E731
     for bad in (dict(dk=None), dict(dsl=one), dict(lse=None), dict(do=None), dict(out=None), dict(v=None), dict(hq=5), dict(dt=3000)):
         assert back(**bad) == _backend.FLK_EINVAL and _backend.last_error(), bad
-    need = lib.flk_attention_backward_workspace_bytes(1, 5, 7, 4, 2, 8, 8, 0, 0)
+    need = lib.flk_attention_backward_workspace_bytes(1, 5, 7, 4, 2, 8, 8, 0, 0, 0)
     assert need > 0 and back(ws=one, wsb=need - 1) == _backend.FLK_ENOMEM
-    assert lib.flk_attention_backward_workspace_bytes(1, 5, 7, 3, 2, 8, 8, 0, 0) == 0
+    assert lib.flk_attention_backward_workspace_bytes(1, 5, 7, 3, 2, 8, 8, 0, 0, 0) == 0
     cnames = "q qb qs qh k kb ks kh v vb vs vh lens b t cap_ hq hk d dv scale cap slopes out dt ws wsb st".split()
     cbase = {**base, "lens": one, "t": 1, "cap_": 100_000}
     cached = lambda **kw: lib.flk_attention_cached(*[{**cbase, **kw}[n] for n in cnames])  # noqa: E731
