@@ -208,14 +208,19 @@ static FwdSizes fwd_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t
     return z;
 }
 
-// Workgroups the keys of a sequence are divided over, none of them with less than four tiles a wave at the cache's capacity.
-// One sequence: two workgroups for each compute unit, which run at once, and no part more to be added than that takes.
-// Several: shorter parts, so that sequences of unequal lengths even out (64 sequences of up to 16384 keys, 8 key heads: 0.43 ms
-// with 4 parts, and 0.47 ms with 1).
+// Workgroups the keys of a sequence are divided over: as many as run at once (two for each compute unit), since every part more
+// is written and added again (8 sequences of up to 8192 keys, 8 key heads: 39 us so, 45 with four times as many; one of 122 000:
+// 60 us and 75), and none with less than four tiles a wave at the cache's capacity;
+// less than four parts do not make up for the second kernel.  Where the sequences alone fill the chip,
+// parts of at most 4096 keys (four at most) even out their lengths (64 of up to 16384 keys: 426 us with 4 parts, 474 undivided;
+// of up to 1024: 39 us with 2, 33 undivided).
 static int cached_splits(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk) {
     const int64_t groups = b * hk * cdiv(t * (hq / hk), 32);
-    const int64_t most = cdiv(capacity, 4 * 4 * kCachedKeys);
-    int64_t n = groups > 0 ? cdiv(b == 1 ? 512 : 2048, groups) : 1;
+    int64_t most = cdiv(capacity, 4 * 4 * kCachedKeys);
+    if (most < 4) most = 1;
+    int64_t n = groups > 0 ? cdiv(512, groups) : 1;
+    const int64_t even = capacity / 4096 < 4 ? capacity / 4096 : 4;
+    if (b > 1 && n < even) n = even;
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }

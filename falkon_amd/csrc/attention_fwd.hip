@@ -87,6 +87,10 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         }
     };
 
+    // Up to four float outputs a row, as a regression has them, would leave most of a matrix instruction's 32 columns empty, each
+    // of them as dear as a column of the scores' product: their sums are made by vector instructions, each half of the
+    // lanes for its keys, in the first four registers of o (1e5 rows of 28 features, 2000 keys, 4 outputs: 326 -> 257 us).
+    const bool few = sizeof(T) == 4 && DP <= 64 && p.dv_d <= 4;     // (wider heads have no registers to spare)
     fx16 o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) o[db] = fx16{};
@@ -194,28 +198,38 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                 s[kb][r] = e;
                 sum[r & 3] += e;
             };
-            constexpr int F = ST * DB, EX = (16 + F - 1) / F;
-            frag vf[F], pf[ST];
+            if (few) {
 #pragma unroll
-            for (int i = 0; i < F; i++) vf[i] = TL::cols(lds_v, at_lane, AT::KS * (i / DB), i % DB);
-            FLK_KEEP_ORDER();
+                for (int r = 0; r < 16; r++) {
+                    weight(0, r);
+                    const fx4 v = *(const fx4 *)(lds_v + TL::at(8 * (r >> 2) + 4 * half + (r & 3), 0));
 #pragma unroll
-            for (int r = 0; r < 16; r++) weight(0, r);
+                    for (int c = 0; c < 4; c++) o[0][c] = __builtin_fmaf(s[0][r], v[c], o[0][c]);
+                }
+            } else {
+                constexpr int F = ST * DB, EX = (16 + F - 1) / F;
+                frag vf[F], pf[ST];
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-#pragma unroll
-                for (int st = 0; st < ST; st++) pf[st] = pack<T>(s[kb], st);
+                for (int i = 0; i < F; i++) vf[i] = TL::cols(lds_v, at_lane, AT::KS * (i / DB), i % DB);
                 FLK_KEEP_ORDER();
 #pragma unroll
-                for (int i = 0; i < F; i++) {
-                    o[i % DB] = AT::mma(vf[i], pf[i / DB], o[i % DB]);
-                    if (kb + 1 < KB) {
-                        vf[i] = TL::cols(lds_v, at_lane, 32 * (kb + 1) + AT::KS * (i / DB), i % DB);
+                for (int r = 0; r < 16; r++) weight(0, r);
 #pragma unroll
-                        for (int r = i * EX; r < (i + 1) * EX; r++)
-                            if (r < 16) weight(kb + 1, r);
-                    }
+                for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+                    for (int st = 0; st < ST; st++) pf[st] = pack<T>(s[kb], st);
                     FLK_KEEP_ORDER();
+#pragma unroll
+                    for (int i = 0; i < F; i++) {
+                        o[i % DB] = AT::mma(vf[i], pf[i / DB], o[i % DB]);
+                        if (kb + 1 < KB) {
+                            vf[i] = TL::cols(lds_v, at_lane, 32 * (kb + 1) + AT::KS * (i / DB), i % DB);
+#pragma unroll
+                            for (int r = i * EX; r < (i + 1) * EX; r++)
+                                if (r < 16) weight(kb + 1, r);
+                        }
+                        FLK_KEEP_ORDER();
+                    }
                 }
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -236,6 +250,10 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         skip = walk.is_skip;
     }
     l += other_half(l);
+    if (few) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[0][c] += other_half(o[0][c]);
+    }
     if (p.parts > 1) {                                             // joined by attention_parts_kernel
         const int64_t rows_all = (int64_t)p.b * p.sq * p.hq, first = ((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h;
         __syncthreads();

@@ -70,6 +70,21 @@ __device__ __forceinline__ A row_sum(A x, A *lds) {
     return x;
 }
 
+// Two sums at once; with four waves a row one barrier suffices if the caller alternates between two places in LDS.
+template <int TPR, typename A>
+__device__ __forceinline__ void row_sums(A &x, A &y, A *lds) {
+#pragma unroll
+    for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) { x += __shfl_xor(x, off, 64); y += __shfl_xor(y, off, 64); }
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) { lds[2 * wave] = x; lds[2 * wave + 1] = y; }
+        __syncthreads();
+        x = y = A(0);
+#pragma unroll
+        for (int w = 0; w < TPR / 64; w++) { x += lds[2 * w]; y += lds[2 * w + 1]; }
+    }
+}
+
 template <typename T> struct NormArgs {
     typedef typename NormAcc<T>::type acc;
     const T *x, *dy;
@@ -164,43 +179,59 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_bwd_kernel(NormArgs<T>
     typedef typename NormArgs<T>::acc A;
     constexpr int kRows = kRowThreads / TPR;
     constexpr int kWidth = TPR * NV * VEC;             // columns a row's threads hold
-    constexpr int kLds = TPR <= 64 ? 2 * kWidth : kRowThreads / 64;
+    constexpr int kLds = TPR <= 64 ? 2 * kWidth : 4 * (kRowThreads / 64);
     __shared__ A lds[kLds];
     const int sub = threadIdx.x % TPR;
     const A inv_d = A(1) / A(p.d);
-    A w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+    A dw[NV][VEC], db[NV][VEC];
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-        if (p.w != nullptr) load_weight<T, VEC, A>(p.w, p.wide, (int64_t)(n * TPR + sub) * VEC, p.d, w[n]);
+    for (int n = 0; n < NV; n++)
 #pragma unroll
-        for (int j = 0; j < VEC; j++) { if (p.w == nullptr) w[n][j] = A(1); dw[n][j] = db[n][j] = A(0); }
-    }
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kRows) {
+        for (int j = 0; j < VEC; j++) dw[n][j] = db[n][j] = A(0);
+    // the next row's values are on their way while the present one's are summed
+    NormVec<T, VEC> nx[NV], ny[NV];
+    A n_mean = A(0), n_rstd = A(0);
+    const auto fetch = [&](int64_t row0) {
+        const int64_t row = row0 + threadIdx.x / TPR, at = row < p.rows ? row : p.rows - 1;
+        n_mean = p.mean[at];
+        n_rstd = p.rstd[at];
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            const int64_t i = (int64_t)(n * TPR + sub) * VEC;
+            if (i < p.d) {
+                nx[n] = *reinterpret_cast<const NormVec<T, VEC> *>(p.x + at * p.x_rs + i);
+                ny[n] = *reinterpret_cast<const NormVec<T, VEC> *>(p.dy + at * p.dy_rs + i);
+            }
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row0 = (int64_t)blockIdx.x * kRows;
+    if (row0 < p.rows) fetch(row0);
+    for (int turn = 0; row0 < p.rows; row0 += step, turn ^= 1) {
         const int64_t row = row0 + threadIdx.x / TPR;
         const bool live = row < p.rows;
-        const int64_t at = live ? row : p.rows - 1;
-        const A mean = p.mean[at], rstd = p.rstd[at];
+        const A mean = n_mean, rstd = n_rstd;
         A z[NV][VEC], g[NV][VEC];
         A s1 = A(0), s2 = A(0);
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             const int64_t i = (int64_t)(n * TPR + sub) * VEC;
-            load_vec<T, VEC, A>(p.x + at * p.x_rs, i, p.d, z[n]);
-            load_vec<T, VEC, A>(p.dy + at * p.dy_rs, i, p.d, g[n]);      // zero past the row's end
-        }
-#pragma unroll
-        for (int n = 0; n < NV; n++) {
+            A w[VEC];
+            if (p.w != nullptr) load_weight<T, VEC, A>(p.w, p.wide, i, p.d, w);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                z[n][j] = (z[n][j] - mean) * rstd;
+                z[n][j] = i < p.d ? (to_acc<A>(nx[n].v[j]) - mean) * rstd : A(0);
+                g[n][j] = i < p.d ? to_acc<A>(ny[n].v[j]) : A(0);
                 if (live) { dw[n][j] += g[n][j] * z[n][j]; db[n][j] += g[n][j]; }
-                g[n][j] *= w[n][j];
+                if (p.w != nullptr) g[n][j] *= w[j];
                 s1 += g[n][j];
                 s2 += g[n][j] * z[n][j];
             }
         }
-        s1 = row_sum<TPR, A>(s1, lds) * inv_d;
-        s2 = row_sum<TPR, A>(s2, lds) * inv_d;
+        if (row0 + step < p.rows) fetch(row0 + step);
+        row_sums<TPR, A>(s1, s2, lds + (TPR > 64 ? turn * 2 * (kRowThreads / 64) : 0));
+        s1 *= inv_d;
+        s2 *= inv_d;
         if (p.y == nullptr || !live) continue;
 #pragma unroll
         for (int n = 0; n < NV; n++) {

@@ -216,6 +216,23 @@ def test_matrices_and_empty_shapes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,m,d,t", [(1000, 500, 28, 1), (300, 2000, 9, 4), (515, 333, 60, 3), (40_000, 70, 28, 2)])
+def test_few_outputs(n, m, d, t):
+    """Kernel smoothing: float rows of one head, a handful of outputs; hidden bad values among them."""
+    q, k, v, do = _make(1, n, m, 1, 1, d, t, torch.float32, seed=22)
+    _check(q, k, v, do)
+    ids = torch.zeros(1, max(n, m), dtype=torch.int32, device=DEV)
+    q, k, v, do = _make(1, min(n, m), m, 1, 1, d, t, torch.float32, seed=23)
+    ids = ids[:, :m]
+    ids[:, m // 2:] = 1
+    clean = _check(q, k, v, do, causal=True, documents=ids)
+    v[:, m - 3, :, t - 1] = float("nan")
+    got = attention(q, k, v, causal=True, documents=ids)
+    assert bool(got[:, -3:, :, t - 1].isnan().all()) and torch.equal(got[:, :-3], clean["out"][:, :-3])
+    assert torch.equal(got[..., :t - 1], clean["out"][..., :t - 1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_extreme_scores(dtype):
     """Scores that a plain exponential would overflow on, one key far above the others, large equal scores."""
