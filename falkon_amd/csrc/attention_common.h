@@ -21,6 +21,8 @@ typedef f16_t hx8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bx8 __attribute__((ext_vector_type(8)));
 typedef short sx4 __attribute__((ext_vector_type(4)));
 typedef unsigned ux4 __attribute__((ext_vector_type(4)));
+typedef ux4 ux4_any2 __attribute__((aligned(2)));          // at any address of a 2 (4) byte value
+typedef ux4 ux4_any4 __attribute__((aligned(4)));
 
 constexpr float kScoreUnit = 1.44269504088896340736f;   // log2(e): scores are kept in units of log 2
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -34,6 +36,7 @@ constexpr int kDocBlock = 32;              // positions one entry of the documen
 template <typename T> struct AttnType;
 template <> struct AttnType<float> {
     typedef fx4 frag;
+    typedef ux4_any4 any;
     static constexpr int E = 4, KS = 8, kTile = 32, M = 4, R = 4;   // M, R: matrix instructions and cross-row reads a fragment
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) {
 #pragma unroll
@@ -44,11 +47,13 @@ template <> struct AttnType<float> {
 };
 template <> struct AttnType<f16_t> {
     typedef hx8 frag;
+    typedef ux4_any2 any;
     static constexpr int E = 8, KS = 16, kTile = 64, M = 1, R = 2;
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct AttnType<bf16_t> {
     typedef bx8 frag;
+    typedef ux4_any2 any;
     static constexpr int E = 8, KS = 16, kTile = 64, M = 1, R = 2;
     static __device__ __forceinline__ fx16 mma(frag a, frag b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -190,12 +195,14 @@ struct AttnArgs {
     int causal, vec;                                   // vec: all rows can be read 16 bytes at a time
 };
 
-// 16 bytes of a row from value c * E on; zero past the row's end.  Rows that are not aligned are read value by value.
+// 16 bytes of a row from value c * E on; zero past the row's end.  The hardware reads them from any address; where a row does not
+// end with a chunk (vec: it does), its last values are read one by one.
 template <typename T> __device__ __forceinline__ ux4 load_chunk(const T *row, int c, int d, bool live, int vec) {
     constexpr int E = AttnType<T>::E;
     ux4 r = {0, 0, 0, 0};
     if (live && c * E < d) {
         if (vec) r = *(const ux4 *)(row + c * E);
+        else if (c * E + E <= d) r = *(const typename AttnType<T>::any *)(row + c * E);
         else {
             union { T t[E]; ux4 u; } x;
             x.u = r;
@@ -212,7 +219,7 @@ template <typename T> __device__ __forceinline__ ux4 load_chunk(const T *row, in
 // a wave's instruction fills 1024 consecutive bytes of LDS, so the permutation of the chunks is applied to the addresses
 // read.  Lanes past the last row or the row's end read out of the buffer's bounds and bring zeros.  The reads are counted by
 // vmcnt; wait() and a barrier stand between them and the tile's use.  Their targets are named by 16 bits, so tiles lie in the first
-// 64 KB of LDS.  Other rows are read value by value.
+// 64 KB of LDS.  Other rows pass through registers.
 constexpr unsigned kNowhere = 0x80000000u;                 // an offset behind every buffer's end
 template <typename T, int DP, int TR> struct Feed {
     typedef Tile<T, DP> TL;
@@ -251,10 +258,20 @@ template <typename T, int DP, int TR> struct Feed {
                              :: "s"(to + n * kAttnThreads * 16), "v"(o), "s"(rsrc), "s"(so) : "memory", "m0");
             }
         } else {
+            constexpr int B = N % 4 == 0 ? 4 : N % 3 == 0 ? 3 : N % 2 == 0 ? 2 : 1;      // reads on their way at once
 #pragma unroll 1
-            for (int n = 0; n < N; n++) {
-                const int i = n * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC;
-                *(ux4 *)(tile + TL::at(row, c)) = load_chunk<T>(base + (row0 + row) * stride, c, d, row < rows, 0);
+            for (int n0 = 0; n0 < N; n0 += B) {
+                ux4 t[B];
+#pragma unroll
+                for (int n = 0; n < B; n++) {
+                    const int i = (n0 + n) * kAttnThreads + threadIdx.x, row = i / NC, c = i % NC;
+                    t[n] = load_chunk<T>(base + (row0 + row) * stride, c, d, row < rows, 0);
+                }
+#pragma unroll
+                for (int n = 0; n < B; n++) {
+                    const int i = (n0 + n) * kAttnThreads + threadIdx.x;
+                    *(ux4 *)(tile + TL::at(i / NC, i % NC)) = t[n];
+                }
             }
         }
     }
@@ -303,6 +320,7 @@ __device__ __forceinline__ void store_rows(char *lds, Part part, T *out, int64_t
         const char *from = lds + TL::at(row, c);
         T *to = out + row * stride + c * E;
         if (vec) *(ux4 *)to = *(const ux4 *)from;
+        else if (c * E + E <= d) *(typename AttnType<T>::any *)to = *(const ux4 *)from;
         else
             for (int j = 0; j < E && c * E + j < d; j++) to[j] = ((const T *)from)[j];
     }
