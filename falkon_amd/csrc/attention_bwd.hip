@@ -372,6 +372,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
             if (!whole && __any(!(__builtin_fabsf(delta_of[lane % TQ]) < kInf))) {   // a row that is not finite, hidden from some keys
                 FD::clean_share(lds_q);
                 FD::clean_share(lds_g);
+                // keys that do see it get weights of NaN for it
+                if (mine && !(__builtin_fabsf(delta_of[threadIdx.x]) < kInf)) lds_stat[buf ^ 1][0][threadIdx.x] = __builtin_nanf("");
                 __syncthreads();
             }
             if (!skip) {
@@ -419,12 +421,10 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                         float grad = 1.f;
                         if constexpr (MOD == kPlain) e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][r], score.unit, -li));
                         else e[k] = __builtin_amdgcn_exp2f(score(s[qb][r], at_row + (float)(32 * qb + 8 * (r >> 2) + (r & 3)), grad) - li);
-                        g[k] = e[k] * (dp[qb][r] - de);
-                        if constexpr ((MOD & kCap) != 0) g[k] *= grad;
-                        if (masked) {
-                            e[k] = seen.or_zero(__builtin_fmaf(de, 0.f, e[k]), qb, r);
-                            g[k] = seen.or_zero(g[k], qb, r);
-                        }
+                        float x = dp[qb][r] - de;
+                        if constexpr ((MOD & kCap) != 0) x *= grad;
+                        if (masked) e[k] = seen.or_zero(e[k], qb, r);
+                        g[k] = times_or_zero(e[k], x);                       // a hidden place stays zero whatever x is
                     }
                     union { frag f; two t[AT::E / 2]; } u, v;
                     const int st = 2 * pair / AT::E, at2 = pair % (AT::E / 2);

@@ -381,6 +381,12 @@ struct Seen {
     }
     __device__ __forceinline__ float or_zero(float x, int kb, int r) const { return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & bits(kb, r)); }
 };
+// a b, and zero where a is zero, also if b is an infinity or a NaN
+__device__ __forceinline__ float times_or_zero(float a, float b) {
+    float c;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(c) : "v"(a), "v"(b));
+    return c;
+}
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 // The places whose id (place l's in lane l) is this lane's: one round for every different id among the lanes, which are few.
 __device__ __forceinline__ uint64_t same_id(int place_id, int id) {

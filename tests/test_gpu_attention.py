@@ -168,6 +168,16 @@ def test_bad_values_in_hidden_places(dtype):
         other = torch.ones(s, dtype=torch.bool, device=DEV)
         other[60:130] = False
         assert all(torch.equal(got[n][:, other], clean[n][:, other]) for n in ("dq", "dk", "dv"))
+        q5, do5 = q.clone(), do.clone()
+        q5[:, 70], do5[:, 100] = float("nan"), value        # keys 60 .. 70, and 60 .. 100, are seen by one of them
+        got = _run(q5, k, v, do5, causal=True, documents=ids)
+        assert bool(got["dk"][:, 60:101].isnan().all()) and bool(got["dv"][:, 60:101].isnan().all())
+        other[60:130] = True
+        other[60:101] = False
+        assert all(torch.equal(got[n][:, other], clean[n][:, other]) for n in ("dk", "dv"))
+        other[60:130] = True
+        other[70] = other[100] = False
+        assert torch.equal(got["dq"][:, other], clean["dq"][:, other]) and bool(got["dq"][:, [70, 100]].isnan().all())
     v4 = v.clone()
     v4[:, 150, :, 3], v4[:, 150, :, 4] = float("inf"), -float("inf")
     out = attention(q, k, v4, causal=True)
