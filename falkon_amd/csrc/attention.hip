@@ -142,6 +142,8 @@ static int attn_check(const char *what, int64_t b, int64_t sq, int64_t sk, int64
     if (d > kAttnMaxD || dv > kAttnMaxD) return fail(FLK_EUNSUPPORTED, "%s: heads of more than %d values", what, kAttnMaxD);
     if (sq > kMaxPositions || sk > kMaxPositions) return fail(FLK_EUNSUPPORTED, "%s: more than %lld positions", what, (long long)kMaxPositions);
     if (!(softcap >= 0.0)) return fail(FLK_EINVAL, "%s: softcap must not be negative", what);
+    if (softcap > 0.0 && (softcap < kMinCap || (dtype != FLK_F32 && softcap > kMaxCap16)))
+        return fail(FLK_EUNSUPPORTED, "%s: softcap of %g (%g to %g for 16-bit data)", what, softcap, kMinCap, kMaxCap16);
     if (prefix != nullptr && !causal) return fail(FLK_EINVAL, "%s: a prefix belongs to a causal mask", what);
     if (docs != nullptr && sq > sk) return fail(FLK_EINVAL, "%s: documents need every query to stand at a key's position", what);
     if (b > 0 && (hq > kMaxGrid / b || b * hq * cdiv(sq > sk ? sq : sk, kAttnRows) > kMaxGrid))
@@ -267,7 +269,8 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
     a.part_o = (float *)ws; ws += z.o;
     a.part_ml = (float *)ws;
     const int es = elem_size(dtype);
-    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) && aligned16(out) && aligned16(a.rest);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es);
+    a.vec_v = rows_aligned(v, a.vs, dv, es) && aligned16(out) && aligned16(a.rest);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);
@@ -316,8 +319,8 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     a.dq_part = (float *)ws; ws += z.dq;
     a.dkv_part = (float *)ws;
     const int es = elem_size(dtype);
-    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es) &&
-            rows_aligned(dout, a.dos, dv, es) && aligned16(out) && aligned16(a.rest) && aligned16(dq) && aligned16(dk) && aligned16(dv_out);
+    a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && aligned16(dq) && aligned16(dk);
+    a.vec_v = rows_aligned(v, a.vs, dv, es) && rows_aligned(dout, a.dos, dv, es) && aligned16(out) && aligned16(a.rest) && aligned16(dv_out);
     hipStream_t st = (hipStream_t)stream;
     if ((rc = launch_docs(a, st)) != FLK_OK) return rc;
     const int dp = padded_d(d > dv ? d : dv);

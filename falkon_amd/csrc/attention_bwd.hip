@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     at_lane.init();
     FD feed_k, feed_v;
     feed_k.init((const T *)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, p.d, p.vec);
-    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec);
+    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec_v);
     const T *qrow = (const T *)p.q + b * p.qs.b + h * p.qs.h + (int64_t)row * p.qs.s;
     const T *grow = (const T *)p.dout + b * p.dos.b + h * p.dos.h + (int64_t)row * p.dos.s;
     const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
@@ -53,9 +53,9 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     for (int c = 0; c < C; c++) {
         union { ux4 u; frag f; } x, g, o, e;
         x.u = load_chunk<T>(qrow, 2 * c + half, p.d, live, p.vec);
-        g.u = load_chunk<T>(grow, 2 * c + half, p.dv_d, live, p.vec);
-        o.u = load_chunk<T>((const T *)p.out + at, 2 * c + half, p.dv_d, live, p.vec);
-        e.u = load_chunk<T>((const T *)p.rest + at, 2 * c + half, p.dv_d, live && p.rest != nullptr, p.vec);
+        g.u = load_chunk<T>(grow, 2 * c + half, p.dv_d, live, p.vec_v);
+        o.u = load_chunk<T>((const T *)p.out + at, 2 * c + half, p.dv_d, live, p.vec_v);
+        e.u = load_chunk<T>((const T *)p.rest + at, 2 * c + half, p.dv_d, live && p.rest != nullptr, p.vec_v);
         qf[c] = x.f;
         gf[c] = g.f;
         bits |= bad_bits<T>(x.u) | bad_bits<T>(g.u);
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     for (int c = 0; c < C; c++) {
         union { ux4 u; frag f; } x, y;
         x.u = load_chunk<T>(krow, 2 * c + half, p.d, live, p.vec);
-        y.u = load_chunk<T>(vrow, 2 * c + half, p.dv_d, live, p.vec);
+        y.u = load_chunk<T>(vrow, 2 * c + half, p.dv_d, live, p.vec_v);
         kf[c] = x.f;
         vf[c] = y.f;
     }
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     Score<T, MOD> score(p.scale, p.cap, 0.f);
     FD feed_q, feed_g;
     feed_q.init((const T *)p.q + b * p.qs.b + (hk * p.group + head) * p.qs.h, p.qs.s, p.d, p.vec);
-    feed_g.init((const T *)p.dout + b * p.dos.b + (hk * p.group + head) * p.dos.h, p.dos.s, p.dv_d, p.vec);
+    feed_g.init((const T *)p.dout + b * p.dos.b + (hk * p.group + head) * p.dos.h, p.dos.s, p.dv_d, p.vec_v);
     const float *stats = p.stats + ((int64_t)b * p.hq + hk * p.group + head) * 2 * p.sq_pad;
     // a tile's statistics (padded to whole tiles of 128 rows) pass through registers of its first threads
     float r_lse = 0.f, r_delta = 0.f;
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     if (splits == 1) {
         char *mine = lds + wave * 32 * TL::RB;
         store_rows<T, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, (T *)p.dk + at_k, row_k, rows, p.d, p.vec);
-        store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r]; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec);
+        store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r]; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec_v);
     } else {                                                       // parts in float, added by attention_join_kernel
         const int64_t nk = (int64_t)p.b * p.sk * row_k, nv = (int64_t)p.b * p.sk * row_v;
         char *mine = lds + wave * 32 * Tile<float, DP>::RB;

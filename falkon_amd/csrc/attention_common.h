@@ -192,7 +192,8 @@ struct AttnArgs {
     int2 *doc_range;                                   // [b][doc_blocks]: smallest and largest id of kDocBlock positions
     int *doc_ids;                                      // [b][doc_blocks * kDocBlock]: the ids, -1 for padding and past the end
     int doc_blocks;
-    int causal, vec;                                   // vec: all rows can be read 16 bytes at a time
+    int causal;
+    int vec, vec_v;                                    // rows of q and k (of v and what is like it) are whole aligned chunks
 };
 
 // 16 bytes of a row from value c * E on; zero past the row's end.  The hardware reads them from any address; where a row does not
@@ -332,8 +333,10 @@ constexpr int kPlain = 0, kCap = 1, kDecay = 2, kCapDecay = 3;
 
 // Scores x in units of log 2, and the derivative of the cap.  With r = 1 / (1 + exp(2 u)), u = scale s / cap:
 // cap tanh u = cap - 2 cap r, and its derivative in u is 4 cap r (1 - r).  Two transcendental instructions a score; r comes with an
-// error of 2^-24, so a score with one of cap 2^-22, far below what rounding the weights to 16 bits costs.  Float data take the odd
+// error of 2^-24, so a score with one of cap 2^-22, far below what rounding the weights to 16 bits costs for caps up to
+// kMaxCap16.  Float data take the odd
 // series instead where tanh is small and 1 - 2 r would cancel (its next term is below 2^-25 of the sum at u = 1/4).
+constexpr double kMaxCap16 = 4096.0, kMinCap = 1e-20;
 template <typename T, int MOD> struct Score {
     static constexpr bool kHasCap = (MOD & 1) != 0, kHasDecay = (MOD & 2) != 0, kWide = sizeof(T) == 4;
     float unit, in, out, slope;

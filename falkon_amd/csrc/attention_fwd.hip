@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     at_lane.init();
     FD feed_k, feed_v;
     feed_k.init((const T *)p.k + b * p.ks.b + hk * p.ks.h, p.ks.s, p.d, p.vec);
-    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec);
+    feed_v.init((const T *)p.v + b * p.vs.b + hk * p.vs.h, p.vs.s, p.dv_d, p.vec_v);
     frag qf[C];
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -273,9 +273,9 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     const int rows = p.sq - (i0 + wave * 32);
     __syncthreads();
     char *mine = lds + wave * 32 * TL::RB;
-    store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r]; }, (T *)p.o + at, row_o, rows, p.dv_d, p.vec);
+    store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r]; }, (T *)p.o + at, row_o, rows, p.dv_d, p.vec_v);
     if (p.rest != nullptr)
-        store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r] - (float)(T)o[db][r]; }, (T *)p.rest + at, row_o, rows, p.dv_d, p.vec);
+        store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r] - (float)(T)o[db][r]; }, (T *)p.rest + at, row_o, rows, p.dv_d, p.vec_v);
     if (!live) return;
     if (half == 0 && p.lse != nullptr)
         p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : m * kLn2 + __logf(l);

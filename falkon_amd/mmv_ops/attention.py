@@ -124,11 +124,14 @@ class _AttentionFn(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, slopes, prefix, documents, out, rest, lse)
         ctx.plain = scale, softcap, causal
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)                   # no tensor of zeros for the gradient that lse does not have
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 9
         q, k, v, slopes, prefix, documents, out, rest, lse = ctx.saved_tensors
         scale, softcap, causal = ctx.plain
         need_q, need_k, need_v, need_slopes = ctx.needs_input_grad[:4]
@@ -170,7 +173,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
         within a row are not next to each other is copied first).
     causal : a row sees keys up to its own position only.
     scale : factor of the inner products, ``1 / sqrt(d)`` by default.
-    softcap : cap of the scores, 0 for none.
+    softcap : cap of the scores, 0 for none; from 1e-20 to 4096 for 16-bit data (whose scores would lose digits to a larger one).
     slopes : float32, one per query head: decay of the score with the distance between a row's and a key's position.
     prefix : (batch,) whole numbers, with ``causal`` only: the first ``prefix[b]`` keys are seen by every row.
     documents : (batch, keys) whole numbers of at most 32 bits: a row sees keys with its own number only, and nothing if that is negative

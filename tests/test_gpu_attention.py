@@ -95,7 +95,7 @@ def test_many_workgroups(dtype, kind, d):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("cap,slope", [(0.0, True), (2.0, False), (30.0, True)])
+@pytest.mark.parametrize("cap,slope", [(0.0, True), (2.0, False), (30.0, True), (4096.0, False)])
 @pytest.mark.parametrize("d", [16, 64, 72, 128])
 def test_capped_and_decaying_scores(dtype, causal, cap, slope, d):
     q, k, v, do = _make(2, 150, 170, 4, 2, d, d, dtype, seed=1)
@@ -510,7 +510,7 @@ def test_c_entry_refusals():
     for bad in (dict(b=-1), dict(hq=0), dict(hq=3), dict(d=0), dict(dt=1), dict(dt=2), dict(cap=-1.0), dict(cap=math.nan), dict(prefix=one),
                 dict(docs=one, sq=9), dict(q=None), dict(k=None), dict(out=None)):
         assert call(**bad) == _backend.FLK_EINVAL and _backend.last_error(), bad
-    for bad in (dict(d=129), dict(dv=129), dict(sk=(1 << 28) + 1), dict(b=1 << 40), dict(b=1 << 20, sq=1 << 28)):
+    for bad in (dict(d=129), dict(dv=129), dict(sk=(1 << 28) + 1), dict(b=1 << 40), dict(b=1 << 20, sq=1 << 28), dict(cap=1e-30), dict(cap=5000.0, dt=4)):
         assert call(**bad) == _backend.FLK_EUNSUPPORTED, bad
     need = lib.flk_attention_workspace_bytes(1, 5, 7, 4, 8, 1, 0)
     assert need > 0 and lib.flk_attention_workspace_bytes(1, 5, 7, 4, 8, 0, 0) == 0
