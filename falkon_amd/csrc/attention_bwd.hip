@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const int pos = row + off, pos_lo = i0 + wave * 32 + off;
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;
     const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
-    const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int prefix = p.prefix != nullptr ? max(min(p.prefix[b], p.sk), 0) : 0;
     const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;
 
     typename TL::Lane at_lane;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int off = p.sk - p.sq;
     const int k0 = tile_k * kAttnRows, k_lo = k0 + wave * 32, key = k_lo + (lane & 31);
     const bool live = key < p.sk;
-    const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int prefix = p.prefix != nullptr ? max(min(p.prefix[b], p.sk), 0) : 0;
     const int first = p.causal && key >= prefix ? key - off : 0;   // first row that sees this key
 
     const T *krow = (const T *)p.k + b * p.ks.b + hk * p.ks.h + (int64_t)key * p.ks.s;

@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     const int pos_end = min(i0 + kAttnRows, p.sq) + off;           // behind the last position of the workgroup
     const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
     constexpr bool kLate = MOD == kPlain || (MOD == kCap && sizeof(T) == 2);   // rising in s: the maximum is looked for before
-    const int prefix = p.prefix != nullptr ? min(p.prefix[b], p.sk) : 0;
+    const int prefix = p.prefix != nullptr ? max(min(p.prefix[b], p.sk), 0) : 0;
     const int last = p.causal ? min(max(pos, prefix - 1), p.sk - 1) : p.sk - 1;   // last key this row sees
 
     const T *qrow = (const T *)p.q + b * p.qs.b + h * p.qs.h + (int64_t)row * p.qs.s;

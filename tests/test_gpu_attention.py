@@ -442,6 +442,14 @@ def test_a_layer_trains_and_then_serves_token_by_token():
             assert float((yi[:, 0] - y[:, i]).norm() / y[:, i].norm()) < 1e-5
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prefix_of_the_lowest_number(dtype):
+    """Counts as none, as every negative one."""
+    q, k, v, do = _make(3, 70, 90, 2, 1, 40, 40, dtype, seed=22)
+    _check(q, k, v, do, causal=True, prefix=torch.tensor([-2 ** 31, -1, 2 ** 31 - 1], device=DEV))
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------------------------------------------------
