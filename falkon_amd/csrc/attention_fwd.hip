@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                         s[kb][r] = score(s[kb][r], at - (float)(32 * kb + 8 * (r >> 2) + (r & 3)), grad);
                     }
             }
-            Seen seen;
+            Seen seen = {{~0u, ~0u}};
             if (!full) {
                 uint64_t see = low_bits(last + 1 - k0);
                 if (p.docs != nullptr) see &= same_id(place_id, id);
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                 else if constexpr (!kLate) e = __builtin_amdgcn_exp2f(s[kb][r] - base_m);
                 else {
                     e = __builtin_amdgcn_exp2f(__builtin_fmaf(score.r(s[kb][r]), -2.f * score.out, score.out - base_m));
-                    e = full || s[kb][r] != -kInf ? e : 0.f;
+                    e = seen.or_zero(e, kb, r);            // (a score of -inf may be seen: the cap makes it finite)
                 }
                 s[kb][r] = e;
                 sum[r & 3] += e;

@@ -450,6 +450,20 @@ def test_prefix_of_the_lowest_number(dtype):
     _check(q, k, v, do, causal=True, prefix=torch.tensor([-2 ** 31, -1, 2 ** 31 - 1], device=DEV))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_scores_that_are_seen_are_capped(dtype):
+    """tanh of an infinite score is one, as it is of a score of thousands, whether or not the key's tile needs a mask."""
+    q, k, v, _ = _make(1, 300, 300, 2, 2, 64, 64, dtype, seed=23)
+    q[..., 0] = torch.where(q[..., 0] < 0, -1.0, 1.0).to(dtype)
+    want, k2 = k.clone(), k.clone()
+    for key, sign in ((0, 1), (70, -1), (150, 1), (299, -1)):
+        want[:, key, :, 0], k2[:, key, :, 0] = sign * 6e4, sign * float("inf")     # 6e4 * 0.2 / 2: tanh is one in any type
+    for kw in (dict(causal=True), dict(), dict(causal=True, slopes=torch.tensor([0.1, 0.0], device=DEV))):
+        got = attention(q, k2, v, scale=0.2, softcap=2.0, **kw)
+        assert bool(got.isfinite().all()) and torch.equal(got, attention(q, want, v, scale=0.2, softcap=2.0, **kw))
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------------------------------------------------
