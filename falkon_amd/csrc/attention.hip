@@ -134,7 +134,7 @@ static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64
     return z;
 }
 
-static int attn_check(const char *what, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, double softcap,
+static int attn_check(const char *what, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, double scale, double softcap,
                       int causal, const int *prefix, const int *docs, int dtype) {
     if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1) return fail(FLK_EINVAL, "%s: bad shape", what);
     if (hq % hk != 0) return fail(FLK_EINVAL, "%s: %lld query heads cannot share %lld key heads evenly", what, (long long)hq, (long long)hk);
@@ -142,8 +142,10 @@ static int attn_check(const char *what, int64_t b, int64_t sq, int64_t sk, int64
     if (d > kAttnMaxD || dv > kAttnMaxD) return fail(FLK_EUNSUPPORTED, "%s: heads of more than %d values", what, kAttnMaxD);
     if (sq > kMaxPositions || sk > kMaxPositions) return fail(FLK_EUNSUPPORTED, "%s: more than %lld positions", what, (long long)kMaxPositions);
     if (!(softcap >= 0.0)) return fail(FLK_EINVAL, "%s: softcap must not be negative", what);
-    if (softcap > 0.0 && (softcap < kMinCap || (dtype != FLK_F32 && softcap > kMaxCap16)))
-        return fail(FLK_EUNSUPPORTED, "%s: softcap of %g (%g to %g for 16-bit data)", what, softcap, kMinCap, kMaxCap16);
+    const double max_cap = dtype == FLK_F32 ? kMaxCap : kMaxCap16;
+    if (softcap > 0.0 && (softcap < kMinCap || softcap > max_cap))
+        return fail(FLK_EUNSUPPORTED, "%s: softcap of %g (%g to %g)", what, softcap, kMinCap, max_cap);
+    if (!(scale >= -kMaxScale && scale <= kMaxScale)) return fail(FLK_EUNSUPPORTED, "%s: scale of %g (at most %g)", what, scale, kMaxScale);
     if (prefix != nullptr && !causal) return fail(FLK_EINVAL, "%s: a prefix belongs to a causal mask", what);
     if (docs != nullptr && sq > sk) return fail(FLK_EINVAL, "%s: documents need every query to stand at a key's position", what);
     if (b > 0 && (hq > kMaxGrid / b || b * hq * cdiv(sq > sk ? sq : sk, kAttnRows) > kMaxGrid))
@@ -250,7 +252,7 @@ int flk_attention(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const vo
                   const int *documents, int64_t documents_b, void *out, void *rest, float *lse, int dtype, void *workspace,
                   size_t workspace_bytes, void *stream) {
     fail(FLK_OK, "%s", "");
-    int rc = attn_check("flk_attention", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
+    int rc = attn_check("flk_attention", b, sq, sk, hq, hk, d, dv, scale, softcap, causal, prefix, documents, dtype);
     if (rc != FLK_OK || b * sq == 0) return rc;
     if (q == nullptr || out == nullptr || (sk > 0 && (k == nullptr || v == nullptr))) return fail(FLK_EINVAL, "flk_attention: null pointer");
     const FwdSizes z = fwd_sizes(b, sq, sk, hq, dv, documents != nullptr, dtype);
@@ -294,7 +296,7 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
                            const int *documents, int64_t documents_b, void *dq, void *dk, void *dv_out, float *dslopes, int dtype,
                            void *workspace, size_t workspace_bytes, void *stream) {
     fail(FLK_OK, "%s", "");
-    int rc = attn_check("flk_attention_backward", b, sq, sk, hq, hk, d, dv, softcap, causal, prefix, documents, dtype);
+    int rc = attn_check("flk_attention_backward", b, sq, sk, hq, hk, d, dv, scale, softcap, causal, prefix, documents, dtype);
     if (rc != FLK_OK) return rc;
     if ((dk == nullptr) != (dv_out == nullptr)) return fail(FLK_EINVAL, "flk_attention_backward: dk and dv come together");
     if (dslopes != nullptr && slopes == nullptr) return fail(FLK_EINVAL, "flk_attention_backward: no slopes to differentiate");
@@ -340,7 +342,7 @@ int flk_attention_cached(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, c
                          int64_t capacity, int64_t hq, int64_t hk, int64_t d, int64_t dv, double scale, double softcap,
                          const float *slopes, void *out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     fail(FLK_OK, "%s", "");
-    int rc = attn_check("flk_attention_cached", b, t, capacity, hq, hk, d, dv, softcap, 1, nullptr, nullptr, dtype);
+    int rc = attn_check("flk_attention_cached", b, t, capacity, hq, hk, d, dv, scale, softcap, 1, nullptr, nullptr, dtype);
     if (rc != FLK_OK || b * t == 0) return rc;
     if (q == nullptr || out == nullptr || lengths == nullptr || (capacity > 0 && (k == nullptr || v == nullptr)))
         return fail(FLK_EINVAL, "flk_attention_cached: null pointer");

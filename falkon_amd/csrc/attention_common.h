@@ -336,7 +336,8 @@ constexpr int kPlain = 0, kCap = 1, kDecay = 2, kCapDecay = 3;
 // error of 2^-24, so a score with one of cap 2^-22, far below what rounding the weights to 16 bits costs for caps up to
 // kMaxCap16.  Float data take the odd
 // series instead where tanh is small and 1 - 2 r would cancel (its next term is below 2^-25 of the sum at u = 1/4).
-constexpr double kMaxCap16 = 4096.0, kMinCap = 1e-20;
+// Within kMaxScale and the caps' limits, 2 log2(e) scale / cap and log2(e) cap are numbers of float.
+constexpr double kMaxCap16 = 4096.0, kMinCap = 1e-20, kMaxCap = 1e20, kMaxScale = 1e18;
 template <typename T, int MOD> struct Score {
     static constexpr bool kHasCap = (MOD & 1) != 0, kHasDecay = (MOD & 2) != 0, kWide = sizeof(T) == 4;
     float unit, in, out, slope;

@@ -13,7 +13,8 @@ sees no key is zero.  Keys that no row sees leave no trace in a result or a grad
 neither does a NaN or an infinity of a key reach a row that does not see it.
 
 Scores, maxima, sums and outputs are held in 32 bits; for 16-bit data the weights (and their gradients) are rounded to
-that type before the second product, which is what the matrix cores take.  Results and gradients are the same run to run.
+that type before the second product, which is what the matrix cores take.  Scores of more than 1e9 in size are beyond statistics
+in 32 bits (a rounding of one is more than an exponent holds): such a row may be NaN.  Results and gradients are the same run to run.
 The reference has no counterpart.  The work is done by ``flk_attention``, ``flk_attention_backward`` and
 ``flk_attention_cached``; nothing is computed on the CPU.
 """
@@ -172,8 +173,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
         GPU tensors of one type: float32, float16 or bfloat16; d and dv up to 128; any strides (a tensor whose values
         within a row are not next to each other is copied first).
     causal : a row sees keys up to its own position only.
-    scale : factor of the inner products, ``1 / sqrt(d)`` by default.
-    softcap : cap of the scores, 0 for none; from 1e-20 to 4096 for 16-bit data (whose scores would lose digits to a larger one).
+    scale : factor of the inner products, ``1 / sqrt(d)`` by default, at most 1e18 in size.
+    softcap : cap of the scores, 0 for none; from 1e-20 to 1e20, or to 4096 for 16-bit data (whose scores would lose digits to a
+        larger one).
     slopes : float32, one per query head: decay of the score with the distance between a row's and a key's position.
     prefix : (batch,) whole numbers, with ``causal`` only: the first ``prefix[b]`` keys are seen by every row.
     documents : (batch, keys) whole numbers of at most 32 bits: a row sees keys with its own number only, and nothing if that is negative

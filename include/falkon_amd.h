@@ -315,7 +315,7 @@ int flk_layer_norm_backward(const void *x, int64_t rows, int64_t d, int64_t x_rs
  * out_i = sum_j softmax_j(x_ij) v_j over the keys j that row i sees, matrix-free, where
  *   x = scale * q_i.k_j;  x <- softcap * tanh(x / softcap) if softcap > 0;  x <- x - slopes[h] * |pos_i - j| if slopes
  * and pos_i = i + sk - sq (the queries are the newest positions).  A row that sees nothing is zero.  softcap: 0, or at
- * least 1e-20 and for 16-bit data at most 4096.
+ * least 1e-20 and at most 1e20, for 16-bit data 4096.  |scale|: at most 1e18.
  * q, k, v: b x rows x heads x values with strides (in elements) of batch, row and head; the values of a row are next to
  * each other.  hq is a multiple of hk; heads up to flk_attention_max_d values.  dtype: FLK_F32, FLK_F16 or FLK_BF16.
  * causal: keys behind pos_i are hidden, except the first prefix[b] of them (prefix: b ints or NULL, causal only).

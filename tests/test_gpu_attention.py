@@ -556,3 +556,33 @@ def test_c_entry_refusals():
     need = lib.flk_attention_cached_workspace_bytes(1, 1, 100_000, 4, 2, 8)
     assert need > 0 and cached(ws=one, wsb=need - 1) == _backend.FLK_ENOMEM
     assert lib.flk_attention_max_d(0) == 128 and lib.flk_attention_max_d(1) == 0
+
+
+def test_c_entries_refuse_scales_and_caps_that_float_cannot_hold():
+    """None of these calls reaches a kernel: the pointers are never read."""
+    from falkon_amd import _backend
+    lib = _backend.load()
+    t = [16, 8, 8, 8]
+    calls = (lambda scale, cap, dt: lib.flk_attention(*t, *t, *t, 1, 5, 7, 4, 2, 8, 8, scale, cap, None, 0, None, None, 0, 16, None, None, dt,
+                                                      None, 0, None),
+             lambda scale, cap, dt: lib.flk_attention_backward(*t, *t, *t, 16, None, 16, *t, 1, 5, 7, 4, 2, 8, 8, scale, cap, None, 0, None, None,
+                                                               0, 16, 16, 16, None, dt, None, 0, None),
+             lambda scale, cap, dt: lib.flk_attention_cached(*t, *t, *t, 16, 1, 1, 9, 4, 2, 8, 8, scale, cap, None, 16, dt, None, 0, None))
+    for call in calls:
+        for scale in (1e39, -1e39, math.inf, math.nan):
+            assert call(scale, 0.0, 0) == _backend.FLK_EUNSUPPORTED and "scale" in _backend.last_error()
+        for cap, dt in ((1e39, 0), (3e38, 0), (math.inf, 0), (1e5, 3), (1e-30, 0)):
+            assert call(1.0, cap, dt) == _backend.FLK_EUNSUPPORTED and "softcap" in _backend.last_error()
+
+
+@pytest.mark.gpu
+def test_the_largest_scales_and_caps():
+    """One key: the score's value is the logarithm of the sum.  A cap of 1e20 leaves a score of about one as it is."""
+    q, k, v, _ = _make(1, 1, 1, 1, 1, 8, 8, torch.float32, seed=24)
+    s = float((q.double() * k.double()).sum())
+    for scale, cap, want in ((1.0, 1e20, s), (1e18, 1e20, 1e20 * math.tanh(s * 1e-2)), (1e18, 1e-20, math.copysign(1e-20, s))):
+        out, lse = attention(q, k, v, scale=scale, softcap=cap, return_lse=True)
+        assert torch.equal(out, v)
+        # eight products with 2^-24 each of sum |q||k|, and 2^-20 for the cap and the units
+        bound = scale * 2.0 ** -21 * float((q * k).abs().sum()) + 2.0 ** -20 * abs(want)
+        assert abs(float(lse) - want) <= (bound if cap != 1e-20 else 2.0 ** -20 * 1e-20)
