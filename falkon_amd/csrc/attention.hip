@@ -212,22 +212,33 @@ static FwdSizes fwd_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t
     return z;
 }
 
-// Workgroups the keys of a sequence are divided over: as many as run at once (two for each compute unit), since every part more
-// is written and added again (8 sequences of up to 8192 keys, 8 key heads: 39 us so, 45 with four times as many; one of 122 000:
-// 60 us and 75), and none with less than four tiles a wave at the cache's capacity;
-// less than four parts do not make up for the second kernel.  Where the sequences alone fill the chip,
+// Workgroups the keys of a sequence are divided over: as many as run at once, since every part more is written and added again and
+// a few workgroups more would be a second round (11 sequences of 8000 keys, 8 key heads of 128: 77 us with 440, 92 with 528; 7 of 16 000 floats,
+// 12 heads of 64: 149 with 504, 198 with 588; but 40 of 4000, 8 heads of 128: 145 with 320, 140 with 640), and none with less than four
+// tiles for each of four waves at the cache's capacity.  At once run two workgroups of four waves on a compute
+// unit; heads above 64 values do better with one of eight (cached_waves), where that leaves few units idle (bf16, heads of 128: 4 key
+// heads and 121 900 keys 52.8 us so, 58.5 with two of four; 8 sequences of 8000 keys, 8 key heads, 47.6 and 49.3.  Heads of 64: 2
+// sequences of 32 000 keys, 8 key heads, 30.6 and 28.9).
+// Less than four parts do not make up for the second kernel.  Where the sequences alone fill the chip,
 // parts of at most 4096 keys (four at most) even out their lengths (64 of up to 16384 keys: 426 us with 4 parts, 474 undivided;
 // of up to 1024: 39 us with 2, 33 undivided).
-static int cached_splits(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk) {
+static int cached_splits(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk, int64_t dv) {
     const int64_t groups = b * hk * cdiv(t * (hq / hk), 32);
     int64_t most = cdiv(capacity, 4 * 4 * kCachedKeys);
     if (most < 4) most = 1;
-    int64_t n = groups > 0 ? cdiv(512, groups) : 1;
+    int64_t n = groups > 0 ? 512 / groups : 1;
+    if (dv > 64 && groups > 0 && 256 / groups * groups >= 240) n = 256 / groups;
     const int64_t even = capacity / 4096 < 4 ? capacity / 4096 : 4;
     if (b > 1 && n < even) n = even;
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
+
+// Waves of a workgroup.  A wave's way through its tiles is what a call takes as long as there is a compute unit for every workgroup, so
+// eight halve it (bf16, 8 key heads of 128, 1000 keys: one sequence 24.5 us with four waves, 16.7 with eight; 32 sequences 26.9 and
+// 25.5); with more workgroups four leave room for two of them on a unit (64 sequences: 45.0 us, and 47.9 with eight).  Up to four
+// tiles give the others nothing to do (100 keys: 5.5 us, and 5.8 with eight).
+static int cached_waves(int64_t workgroups, int64_t capacity) { return workgroups <= 256 && capacity > 4 * kCachedKeys ? 8 : 4; }
 
 }  // namespace flk
 
@@ -333,7 +344,7 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
 
 size_t flk_attention_cached_workspace_bytes(int64_t b, int64_t t, int64_t capacity, int64_t hq, int64_t hk, int64_t dv) {
     if (b < 0 || t < 0 || capacity < 0 || hq < 1 || hk < 1 || dv < 1 || hq % hk != 0) return 0;
-    const int64_t n = cached_splits(b, t, capacity, hq, hk);
+    const int64_t n = cached_splits(b, t, capacity, hq, hk, dv);
     return n > 1 ? align256((size_t)(b * t * hq * n * dv) * 4) + align256((size_t)(b * t * hq * n * 2) * 4) : 0;
 }
 
@@ -346,7 +357,7 @@ int flk_attention_cached(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, c
     if (rc != FLK_OK || b * t == 0) return rc;
     if (q == nullptr || out == nullptr || lengths == nullptr || (capacity > 0 && (k == nullptr || v == nullptr)))
         return fail(FLK_EINVAL, "flk_attention_cached: null pointer");
-    const int64_t n = cached_splits(b, t, capacity, hq, hk);
+    const int64_t n = cached_splits(b, t, capacity, hq, hk, dv);
     const size_t need = flk_attention_cached_workspace_bytes(b, t, capacity, hq, hk, dv);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
@@ -359,6 +370,7 @@ int flk_attention_cached(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, c
     a.b = (int)b; a.t = (int)t; a.capacity = (int)capacity; a.hq = (int)hq; a.hk = (int)hk; a.group = (int)(hq / hk); a.d = (int)d;
     a.dv_d = (int)dv; a.splits = (int)n; a.blocks_r = (int)cdiv(t * (hq / hk), 32); a.scale = (float)scale; a.cap = (float)softcap;
     const int64_t grid = b * hk * a.blocks_r * n;
+    a.waves = cached_waves(grid, capacity);
     if (grid > kMaxGrid || b * t * hq > kMaxGrid) return fail(FLK_EUNSUPPORTED, "flk_attention_cached: too many rows for one launch");
     const int es = elem_size(dtype);
     a.vec = rows_aligned(q, a.qs, d, es) && rows_aligned(k, a.ks, d, es) && rows_aligned(v, a.vs, dv, es);

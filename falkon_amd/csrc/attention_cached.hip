@@ -2,23 +2,24 @@
 //
 // Bound by reading the cache once.  The query rows that read the same keys (the heads that share a key head, times the new
 // tokens) are packed into the 32 columns of the matrix instructions, so that products cost little beside the reads, and the
-// keys of a sequence are divided over workgroups and over a workgroup's four waves.  Every wave walks over tiles of 32 keys of
+// keys of a sequence are divided over workgroups and over a workgroup's four or eight waves.  Every wave walks over tiles of 32 keys of
 // its own with no barrier: the next tile's reads are in flight, in registers, while the present one is used from LDS.  The waves'
 // results meet in LDS, those of several workgroups in a second kernel, both in a fixed order.
 #include "attention_common.h"
 
 namespace flk {
 
-template <typename T, int DP, int MOD>
-__global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) attention_cached_kernel(CachedArgs p) {
+template <typename T, int DP, int MOD, int W>
+__global__ void __launch_bounds__(64 * W, W > 4 || (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_cached_kernel(CachedArgs p) {
     typedef AttnType<T> AT;
     typedef typename AT::frag frag;
     typedef Tile<T, DP> TL;
     constexpr int TK = kCachedKeys, C = DP / AT::KS, DB = DP / 32, ST = 32 / AT::KS, NC = TL::NC, N = TK * NC / 64;
     constexpr int kWave = 2 * TK * TL::RB, kJoin = 32 * (DP + 1) * 4;          // LDS of a wave: its tiles, later its output
     constexpr int kLds = kWave > kJoin ? kWave : kJoin;
-    __shared__ __align__(16) char lds[4 * kLds];
-    __shared__ float lds_ml[4][32][2];
+    __shared__ __align__(16) char lds[W * kLds];
+    __shared__ float lds_ml[W][32][2];
+    static_assert(W * (kLds + 256) <= 160 * 1024, "LDS of a workgroup");
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int pairs = p.b * p.hk;
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     };
     int tile = tile_lo + wave;
     if (tile < tile_hi) fetch(tile);
-    for (; tile < tile_hi; tile += 4) {
+    for (; tile < tile_hi; tile += W) {
         const int k0 = tile * TK;
         const bool full = k0 + TK - 1 <= pos_lo;
         bool bad = false;
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (tile + 4 < tile_hi) fetch(tile + 4);
+        if (tile + W < tile_hi) fetch(tile + W);
         fx16 s = {};
 #pragma unroll
         for (int c = 0; c < C; c++) s = AT::mma(TL::rows(lds_k, at_lane, 0, c), qf[c], s);
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     }
     l += other_half(l);
 
-    // the four waves' results: o relative to the largest of their maxima
+    // the waves' results: o relative to the largest of their maxima
     float *mine = (float *)(lds + wave * kLds);
     __syncthreads();
 #pragma unroll
@@ -143,13 +144,15 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         for (int i = 0; i < 16; i++) mine[(lane & 31) * (DP + 1) + 32 * db + 8 * (i >> 2) + 4 * half + (i & 3)] = o[db][i];
     if (half == 0) { lds_ml[wave][lane][0] = m; lds_ml[wave][lane][1] = l; }
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * DP; i += kAttnThreads) {
+    for (int i = threadIdx.x; i < 32 * DP; i += 64 * W) {
         const int rr = i / DP, c = i % DP, row = rb * 32 + rr;
         if (row >= n_rows || c >= p.dv_d) continue;
-        const float top = fmaxf(fmaxf(lds_ml[0][rr][0], lds_ml[1][rr][0]), fmaxf(lds_ml[2][rr][0], lds_ml[3][rr][0]));
+        float top = lds_ml[0][rr][0];
+#pragma unroll
+        for (int w = 1; w < W; w++) top = fmaxf(top, lds_ml[w][rr][0]);
         float x = 0.f, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
             const float mw = lds_ml[w][rr][0];
             if (mw == -kInf && lds_ml[w][rr][1] == 0.f) continue;  // saw nothing
             const float a = mw == -kInf ? 1.f : __builtin_amdgcn_exp2f(mw - top);
@@ -215,9 +218,28 @@ __global__ void __launch_bounds__(THREADS) attention_cached_join_kernel(CachedAr
     ((T *)p.out)[row * p.dv_d + c] = (T)(sum == 0.f ? 0.f : x / sum);
 }
 
+template <typename T, int DP, int W> void launch_cached_waves(const CachedArgs &a, int kind, dim3 grid, hipStream_t st) {
+    if (kind == kPlain) hipLaunchKernelGGL((attention_cached_kernel<T, DP, kPlain, W>), grid, dim3(64 * W), 0, st, a);
+    else if (kind == kCap) hipLaunchKernelGGL((attention_cached_kernel<T, DP, kCap, W>), grid, dim3(64 * W), 0, st, a);
+    else if (kind == kDecay) hipLaunchKernelGGL((attention_cached_kernel<T, DP, kDecay, W>), grid, dim3(64 * W), 0, st, a);
+    else hipLaunchKernelGGL((attention_cached_kernel<T, DP, kCapDecay, W>), grid, dim3(64 * W), 0, st, a);
+}
+template <typename T, int DP> void launch_cached_kind(const CachedArgs &a, int kind, dim3 grid, hipStream_t st) {
+    constexpr bool kRoom = sizeof(T) == 2 || DP <= 64;             // eight waves' tiles fit into 160 KB of LDS
+    if constexpr (kRoom) {
+        if (a.waves == 8) { launch_cached_waves<T, DP, 8>(a, kind, grid, st); return; }
+    }
+    launch_cached_waves<T, DP, 4>(a, kind, grid, st);
+}
+
 template <typename T> int launch_attention_cached(const CachedArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.blocks_r * a.splits));
-    FLK_ATTN_LAUNCH(attention_cached_kernel, grid)
+    const int kind = score_kind(a.scale, a.cap, a.slopes);
+    if (dp == 32) launch_cached_kind<T, 32>(a, kind, grid, st);
+    else if (dp == 64) launch_cached_kind<T, 64>(a, kind, grid, st);
+    else if (dp == 96) launch_cached_kind<T, 96>(a, kind, grid, st);
+    else launch_cached_kind<T, 128>(a, kind, grid, st);
+    FLK_LAUNCH_CHECK("attention_cached_kernel");
     if (a.splits > 1) {
         const dim3 rows((unsigned)((int64_t)a.b * a.t * a.hq));
         if (a.splits > 16) hipLaunchKernelGGL((attention_cached_join_kernel<T, 1024>), rows, dim3(1024), 0, st, a);

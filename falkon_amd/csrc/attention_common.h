@@ -468,6 +468,7 @@ struct CachedArgs {
     const float *slopes;
     float *part_o, *part_ml;               // parts of several workgroups: [row][split][dv] and [row][split][2]
     int b, t, capacity, hq, hk, group, d, dv_d, splits, blocks_r;
+    int waves;                             // of a workgroup: 4, or 8 where their tiles fit into LDS
     float scale, cap;
     int vec;
 };

@@ -374,6 +374,21 @@ def test_cached(dtype, hq, hk, d, dv, t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,capacity,d,t", [(32, 300, 64, 1), (33, 300, 64, 1), (32, 300, 128, 1), (33, 300, 128, 1), (5, 128, 40, 2),
+                                            (5, 129, 40, 2), (33, 160, 8, 3), (17, 260, 96, 20)])
+def test_cached_on_both_sides_of_the_launch_rules(b, capacity, d, t, dtype):
+    """Eight key heads: 256 workgroups and more, caches of four tiles and more, two blocks of rows for a key head."""
+    lens = [(37 * i + 5) % (capacity + 1) if i % 7 else (0, 1, capacity)[i // 7 % 3] for i in range(b)]
+    q, k, v, _ = _make(b, t, capacity, 16, 8, d, d, dtype, seed=25)
+    for i, n in enumerate(lens):
+        k[i, n:], v[i, n:] = float("nan"), float("inf")
+    got = cached_attention(q, k, v, torch.tensor(lens, device=DEV), softcap=8.0)
+    check({"out": got}, {"out": _cached_reference(q, k, v, lens, softcap=8.0)}, ["out"])
+    assert torch.equal(cached_attention(q, k, v, torch.tensor(lens, device=DEV), softcap=8.0), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_cached_long_and_hidden(dtype):
     """One long sequence over many workgroups; a new token's bad value does not reach the tokens before it."""
     q, k, v, _ = _make(1, 4, 9000, 4, 2, 64, 64, dtype, seed=15)
