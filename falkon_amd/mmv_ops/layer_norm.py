@@ -110,6 +110,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
         if t.shape != x.shape[-1:]:
             raise ValueError(f"{name} must have {x.shape[-1]} entries, got shape {tuple(t.shape)}")
         if t.device != x.device:

@@ -249,3 +249,10 @@ def test_c_entry_refusals():
     assert need > 0
     assert lib.flk_layer_norm_backward(one, 100, 8, 8, one, 8, one, 0, one, one, one, one, one, 0, one, need - 1, None) == _backend.FLK_ENOMEM
     assert lib.flk_layer_norm_backward(one, 100, 8, 8, None, 8, one, 0, one, one, one, one, one, 0, one, need, None) == _backend.FLK_EINVAL
+
+
+def test_refuses_a_weight_that_is_no_tensor():
+    x = torch.zeros(3, 4)
+    for kw in (dict(weight=1.0), dict(bias=[0.0] * 4), dict(weight=torch.ones(4), bias=2)):
+        with pytest.raises(TypeError, match="must be a tensor"):
+            falkon_amd.layer_norm(x, **kw)
