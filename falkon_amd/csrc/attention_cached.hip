@@ -70,17 +70,20 @@ __global__ void __launch_bounds__(64 * W, W > 4 || (sizeof(T) == 4 && DP > 64) ?
         const int k0 = tile * TK;
         const bool full = k0 + TK - 1 <= pos_lo;
         bool bad = false;
+        if (!full) {
+#pragma unroll
+            for (int n = 0; n < N; n++) bad |= any_nonfinite<T>(rv[n]);
+        }
+        const bool careful = !full && __any(bad);
+        if (careful) {                                             // clear them for the product, and add what they do to it below
+#pragma unroll
+            for (int n = 0; n < N; n++) rv[n] = cleaned<T>(rv[n]); // (here, not in LDS: there a lane's 16 bytes are another lane's)
+        }
 #pragma unroll
         for (int n = 0; n < N; n++) {
             const int i = n * 64 + lane, row = i / NC, c = i % NC;
             *(ux4 *)(lds_k + TL::at(row, c)) = rk[n];
             *(ux4 *)(lds_v + TL::at(row, c)) = rv[n];
-            if (!full) bad |= any_nonfinite<T>(rv[n]);
-        }
-        const bool careful = !full && __any(bad);
-        if (careful) {                                             // clear them for the product, and add what they do to it below
-#pragma unroll
-            for (int n = 0; n < N; n++) clean<T>(lds_v + (n * 64 + lane) * 16);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();

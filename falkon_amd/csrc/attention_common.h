@@ -139,15 +139,18 @@ template <typename T> __device__ __forceinline__ typename AttnType<T>::frag pack
 }
 
 // Infinities and NaNs of a tile must not reach rows that hide them, but a product with weight zero would carry them there.
-// They are set to zero in LDS where a mask is needed; clean() does it to this thread's 16 bytes.
-template <typename T> __device__ __forceinline__ void clean(char *at) {
+// They are set to zero where a mask is needed; cleaned() does it to 16 bytes, clean() to this thread's 16 bytes of LDS.
+template <typename T> __device__ __forceinline__ ux4 cleaned(ux4 u) {
     union { ux4 u; T t[16 / sizeof(T)]; } x;
-    x.u = *(const ux4 *)at;
-    if (!any_nonfinite<T>(x.u)) return;
+    x.u = u;
 #pragma unroll
     for (int i = 0; i < (int)(16 / sizeof(T)); i++)
         if (!(__builtin_fabsf((float)x.t[i]) < kInf)) x.t[i] = (T)0.f;
-    *(ux4 *)at = x.u;
+    return x.u;
+}
+template <typename T> __device__ __forceinline__ void clean(char *at) {
+    const ux4 u = *(const ux4 *)at;
+    if (any_nonfinite<T>(u)) *(ux4 *)at = cleaned<T>(u);
 }
 // What they add to the rows that see them: value (key, c), read again from memory, for every output column c this lane holds,
 // where the row's weight is not zero.  w[kb][r]: weights of key 32 kb + 8 (r / 4) + 4 half + r % 4.  Rare, and not made to be
