@@ -126,10 +126,10 @@ __global__ void __launch_bounds__(64 * W, W > 4 || (sizeof(T) == 4 && DP > 64) ?
             }
         }
         if (careful) {
-            fx16 w = s, x[DB];
+            fx16 x[DB];
 #pragma unroll
             for (int db = 0; db < DB; db++) x[db] = o[db];
-            spread_nonfinite<T, 1, DB>(vbase + k0 * p.vs.s, p.vs.s, len - k0, p.dv_d, &w, x);
+            spread_nonfinite<T, TK, DB>(vbase + k0 * p.vs.s, p.vs.s, len - k0, p.dv_d, seen_from(low_bits(pos + 1 - k0)), 1.f, x);
 #pragma unroll
             for (int db = 0; db < DB; db++) o[db] = x[db];
         }

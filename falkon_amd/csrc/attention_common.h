@@ -152,29 +152,6 @@ template <typename T> __device__ __forceinline__ void clean(char *at) {
     const ux4 u = *(const ux4 *)at;
     if (any_nonfinite<T>(u)) *(ux4 *)at = cleaned<T>(u);
 }
-// What they add to the rows that see them: value (key, c), read again from memory, for every output column c this lane holds,
-// where the row's weight is not zero.  w[kb][r]: weights of key 32 kb + 8 (r / 4) + 4 half + r % 4.  Rare, and not made to be
-// fast; called with copies, so that weights and output stay in registers elsewhere.
-template <typename T, int KB, int DB>
-__device__ __noinline__ void spread_nonfinite(const T *rows, int64_t stride, int n, int d, const fx16 *w, fx16 *o) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    for (int key = 0; key < min(n, 32 * KB); key++) {
-        const T *row = rows + key * stride;
-        bool bad = false;
-        for (int c = lane; c < d; c += 64) bad |= !(__builtin_fabsf((float)row[c]) < kInf);
-        if (!__any(bad)) continue;
-        float x = w[key >> 5][4 * (key >> 3 & 3) + (key & 3)];
-        const float y = __shfl_xor(x, 32, 64);
-        x = (key >> 2 & 1) == half ? x : y;
-        for (int db = 0; db < DB; db++)
-            for (int r = 0; r < 16; r++) {
-                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                const float v = c < d ? (float)row[c] : 0.f;
-                if (x != 0.f && !(__builtin_fabsf(v) < kInf)) o[db][r] += v;
-            }
-    }
-}
-
 struct AttnStride { int64_t b, s, h; };
 struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
@@ -410,6 +387,29 @@ __device__ __forceinline__ uint64_t same_id(int place_id, int id) {
 __device__ __forceinline__ Seen seen_from(uint64_t m) {
     m >>= 4 * (threadIdx.x >> 5 & 1);
     return {{(unsigned)m, (unsigned)(m >> 32)}};
+}
+
+// What the values that clean() took from a tile (its first `n` rows) do to the rows that see them: each, read again from memory, times
+// `weight` is added to its column.  With 1 an infinity stays one, however small its weight (0 times it would be a NaN); with 0 it
+// gives the NaN of weights that are zero whenever they are finite.  Rare, and not made to be fast; called with copies, so that the
+// output stays in registers elsewhere.
+template <typename T, int TK, int DB>
+__device__ __noinline__ void spread_nonfinite(const T *rows, int64_t stride, int n, int d, Seen seen, float weight, fx16 *o) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const unsigned w[2] = {(unsigned)__shfl((int)seen.w[0], lane & 31, 64), (unsigned)__shfl((int)seen.w[1], lane & 31, 64)};  // not shifted
+    for (int place = 0; place < min(n, TK); place++) {
+        const T *row = rows + place * stride;
+        bool bad = false;
+        for (int c = lane; c < d; c += 64) bad |= !(__builtin_fabsf((float)row[c]) < kInf);
+        if (!__any(bad)) continue;
+        const bool mine = (place < 32 ? w[0] : w[1]) >> (place & 31) & 1;
+        for (int db = 0; db < DB; db++)
+            for (int r = 0; r < 16; r++) {
+                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
+                const float v = c < d ? (float)row[c] : 0.f;
+                if (mine && !(__builtin_fabsf(v) < kInf)) o[db][r] += v * weight;
+            }
+    }
 }
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }

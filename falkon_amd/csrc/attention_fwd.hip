@@ -158,11 +158,14 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                         s[kb][r] = score(s[kb][r], at - (float)(32 * kb + 8 * (r >> 2) + (r & 3)), grad);
                     }
             }
-            Seen seen = {{~0u, ~0u}};
-            if (!full) {
+            const auto look_at = [&]() {
                 uint64_t see = low_bits(last + 1 - k0);
                 if (p.docs != nullptr) see &= same_id(place_id, id);
-                seen = seen_from(see);
+                return seen_from(see);
+            };
+            Seen seen = {{~0u, ~0u}};
+            if (!full) {
+                seen = look_at();
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -234,12 +237,10 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if (careful) {
-                fx16 w[KB], x[DB];
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++) w[kb] = s[kb];
+                fx16 x[DB];
 #pragma unroll
                 for (int db = 0; db < DB; db++) x[db] = o[db];
-                spread_nonfinite<T, KB, DB>(feed_v.base + k0 * feed_v.stride, feed_v.stride, p.sk - k0, p.dv_d, w, x);
+                spread_nonfinite<T, TK, DB>(feed_v.base + k0 * feed_v.stride, feed_v.stride, p.sk - k0, p.dv_d, seen, 1.f, x);
 #pragma unroll
                 for (int db = 0; db < DB; db++) o[db] = x[db];
             }

@@ -33,3 +33,18 @@ def test_bad_values_anywhere_in_a_cached_row(dtype, d, dv):
         hit = torch.eye(dv, dtype=torch.bool, device=DEV)[:, None].expand(dv, 2, dv)
         assert bool((got[:, 1][hit].isnan() if value != value else got[:, 1][hit] == value).all())
         assert bool(got[:, 1][~hit].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_infinite_value_with_a_weight_of_nothing(dtype):
+    """exp(-300) is zero in 32 bits, and zero times an infinity is no number of any result: rows that see it say so in tiles with
+    a mask and without one, and in that column alone."""
+    q, k, v, _ = _make(1, 200, 200, 2, 2, 64, 64, dtype, seed=31)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[:, [5, 150], :, 0] = -300.0 * 8                                       # the scale is 1 / 8
+    v[:, 5, :, 7], v[:, 150, :, 9] = float("inf"), -float("inf")
+    for out in (attention(q, k, v, causal=True), cached_attention(q, k, v, torch.tensor([200], device=DEV))):
+        assert not bool(out[:, 5:, :, 7].isfinite().any()) and not bool(out[:, 150:, :, 9].isfinite().any())
+        out[:, 5:, :, 7], out[:, 150:, :, 9] = 0.0, 0.0
+        assert bool(out.isfinite().all())
