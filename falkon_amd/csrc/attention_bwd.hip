@@ -23,6 +23,8 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ int lds_doc[8];
     __shared__ float lds_sum[4];
+    __shared__ int lds_bad;
+    __shared__ Spoilt<DP> lds_spoilt[kAttnRows];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int heads = p.b * p.hq, pairs = p.b * p.hk;
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
     const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
+    if (threadIdx.x == 0) lds_bad = 0;
     if (p.docs != nullptr) {
         const int raw = live ? ids[pos] : -1;
         span = {wave_min(raw), wave_max(raw)};
@@ -120,8 +123,78 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         const int k = t * TK + lane;
         return lane < TK && k < p.sk ? ids[k] : -1;
     };
+    bool whole, full, skip;
+    // A tile's part of the sums.  `careful`: its keys' infinities and NaNs are set to zero between the scores, which are formed from
+    // them as they are, and the product with the scores' gradients.
+    const auto visit = [&](int k0, char *lds_k, const char *lds_v, auto careful) __attribute__((always_inline)) {
+        Seen seen = {{~0u, ~0u}};
+        if (!full) {
+            uint64_t see = low_bits(last + 1 - k0);
+            if (p.docs != nullptr) see &= same_id(place_id, id);
+            seen = seen_from(see);
+        }
+        const float at_key = (float)(pos - k0 - 4 * half);
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++) {
+            fx16 s = {}, dp = {};
+            {   // fragments of keys and values, read up to four steps ahead of their products
+                constexpr int W = C < 4 ? C : sizeof(T) == 2 && DP > 96 ? 2 : 4;     // (as the registers allow)
+                frag kf[W], vf[W];
+#pragma unroll
+                for (int i = 0; i < W; i++) { kf[i] = TL::rows(lds_k, at_lane, 32 * kb, i); vf[i] = TL::rows(lds_v, at_lane, 32 * kb, i); }
+                FLK_KEEP_ORDER();
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    s = AT::mma(kf[c % W], qf[c], s);
+                    dp = AT::mma(vf[c % W], gf[c], dp);
+                    if (c + W < C) { kf[c % W] = TL::rows(lds_k, at_lane, 32 * kb, c + W); vf[c % W] = TL::rows(lds_v, at_lane, 32 * kb, c + W); }
+                    FLK_KEEP_ORDER();
+                }
+            }
+            if constexpr (decltype(careful)::value) {
+                if (!whole) FD::clean_block(lds_k, kb);
+            }
+            constexpr int F = ST * DB, WF = F < 4 ? F : 4;
+            frag kt[WF], ds;
+#pragma unroll
+            for (int i = 0; i < WF; i++) kt[i] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * (i / DB), i % DB);
+            FLK_KEEP_ORDER();
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float e, g, grad = 1.f;
+                const float dist = at_key - (float)(32 * kb + 8 * (r >> 2) + (r & 3));
+                if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse));
+                else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse);
+                g = e * (dp[r] - delta);
+                if (!full) g = seen.or_zero(g, kb, r);
+                if constexpr ((MOD & kDecay) != 0 && !decltype(careful)::value) {
+                    if (p.dslopes_part != nullptr) {
+                        if (!full) e = seen.or_zero(e, kb, r);
+                        far += g * __builtin_fabsf(dist);
+                        left += g;
+                        reach += e * __builtin_fabsf(dist);
+                    }
+                }
+                if constexpr ((MOD & kCap) != 0) g *= grad;
+                s[r] = g;
+            }
+            FLK_KEEP_ORDER();
+#pragma unroll
+            for (int i = 0; i < F; i++) {
+                if (i % DB == 0) ds = pack<T>(s, i / DB);
+                acc[i % DB] = AT::mma(kt[i % WF], ds, acc[i % DB]);
+                if (i + WF < F) kt[i % WF] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * ((i + WF) / DB), (i + WF) % DB);
+                FLK_KEEP_ORDER();
+            }
+        }
+        if constexpr (decltype(careful)::value) {
+            // (a score's gradient is zero, because its weight or the cap's derivative is, or NaN where its key is not finite)
+            if (!whole) lds_spoilt[wave * 32 + (lane & 31)].note(feed_k.base + k0 * feed_k.stride, feed_k.stride, min(TK, p.sk - k0), p.d, seen);
+        }
+    };
     int buf = 0, tile = walk.next(look);
-    bool whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
+    whole = walk.is_whole, full = walk.is_full, skip = walk.is_skip;
+    bool bad = false;                                              // a key that is not finite, hidden from some row of the workgroup
     if (tile >= 0) {
         feed_k.issue(lds, tile * TK, min(TK, p.sk - tile * TK));
         feed_v.issue(lds + kTileBytes, tile * TK, min(TK, p.sk - tile * TK));
@@ -140,73 +213,37 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
             feed_v.issue(lds + buf * 2 * kTileBytes + kTileBytes, next * TK, min(TK, p.sk - next * TK));
             if (p.docs != nullptr) next_id = id_at(next);
         }
-        if (!whole) {                                              // a row that sees what this removes has a lse of NaN
-            FD::clean_share(lds_k);
-            __syncthreads();
-        }
-        if (!skip) {
-            Seen seen;
-            if (!full) {
-                uint64_t see = low_bits(last + 1 - k0);
-                if (p.docs != nullptr) see &= same_id(place_id, id);
-                seen = seen_from(see);
-            }
-            const float at_key = (float)(pos - k0 - 4 * half);
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                fx16 s = {}, dp = {};
-                {   // fragments of keys and values, read up to four steps ahead of their products
-                    constexpr int W = C < 4 ? C : sizeof(T) == 2 && DP > 96 ? 2 : 4;     // (as the registers allow)
-                    frag kf[W], vf[W];
-#pragma unroll
-                    for (int i = 0; i < W; i++) { kf[i] = TL::rows(lds_k, at_lane, 32 * kb, i); vf[i] = TL::rows(lds_v, at_lane, 32 * kb, i); }
-                    FLK_KEEP_ORDER();
-#pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        s = AT::mma(kf[c % W], qf[c], s);
-                        dp = AT::mma(vf[c % W], gf[c], dp);
-                        if (c + W < C) { kf[c % W] = TL::rows(lds_k, at_lane, 32 * kb, c + W); vf[c % W] = TL::rows(lds_v, at_lane, 32 * kb, c + W); }
-                        FLK_KEEP_ORDER();
-                    }
-                }
-                constexpr int F = ST * DB, WF = F < 4 ? F : 4;
-                frag kt[WF], ds;
-#pragma unroll
-                for (int i = 0; i < WF; i++) kt[i] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * (i / DB), i % DB);
-                FLK_KEEP_ORDER();
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    float e, g, grad = 1.f;
-                    const float dist = at_key - (float)(32 * kb + 8 * (r >> 2) + (r & 3));
-                    if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse));
-                    else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse);
-                    g = e * (dp[r] - delta);
-                    if (!full) g = seen.or_zero(g, kb, r);
-                    if constexpr ((MOD & kDecay) != 0) {
-                        if (p.dslopes_part != nullptr) {
-                            if (!full) e = seen.or_zero(e, kb, r);
-                            far += g * __builtin_fabsf(dist);
-                            left += g;
-                            reach += e * __builtin_fabsf(dist);
-                        }
-                    }
-                    if constexpr ((MOD & kCap) != 0) g *= grad;
-                    s[r] = g;
-                }
-                FLK_KEEP_ORDER();
-#pragma unroll
-                for (int i = 0; i < F; i++) {
-                    if (i % DB == 0) ds = pack<T>(s, i / DB);
-                    acc[i % DB] = AT::mma(kt[i % WF], ds, acc[i % DB]);
-                    if (i + WF < F) kt[i % WF] = TL::cols(lds_k, at_lane, 32 * kb + AT::KS * ((i + WF) / DB), (i + WF) % DB);
-                    FLK_KEEP_ORDER();
-                }
-            }
-        }
+        if (!whole) bad |= FD::nonfinite(lds_k);
+        if (!skip) visit(k0, lds_k, lds_v, std::false_type{});
         tile = next;
         whole = walk.is_whole;
         full = walk.is_full;
         skip = walk.is_skip;
+    }
+    // Such keys' part of the last product reached rows that hide them: it is formed again from all tiles, one at a time.  (In a loop of
+    // its own: a branch in the middle of the one above takes hundreds of its registers to memory.  The slopes' sums stand: they have no
+    // product with the keys, and are masked.)
+    if (bad) lds_bad = 1;
+    __syncthreads();
+    const bool again = p.dq != nullptr && lds_bad != 0;
+    if (again) {
+#pragma unroll
+        for (int db = 0; db < DB; db++) acc[db] = fx16{};
+        lds_spoilt[wave * 32 + (lane & 31)].clear();
+        walk.start((int)(tiles_k * part / p.parts), (int)(tiles_k * (part + 1) / p.parts));
+        while ((tile = walk.next(look)) >= 0) {
+            const int k0 = tile * TK, n = min(TK, p.sk - k0);
+            __syncthreads();                                       // the tile before has been read
+            feed_k.issue(lds, k0, n);
+            feed_v.issue(lds + kTileBytes, k0, n);
+            if (p.docs != nullptr) place_id = id_at(tile);
+            whole = walk.is_whole;
+            full = walk.is_full;
+            FD::wait();
+            __syncthreads();
+            at_lane.renew();
+            visit(k0, lds, lds + kTileBytes, std::true_type{});    // (a wave that sees nothing of it takes part in the barriers)
+        }
     }
     if ((MOD & kDecay) != 0 && p.dslopes_part != nullptr) {                        // in a fixed order: lanes, then waves
         far += other_half(far);
@@ -222,6 +259,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     }
     if (p.dq == nullptr) return;
     __syncthreads();
+    if (again) lds_spoilt[wave * 32 + (lane & 31)].mark(acc);
     const float unscale = p.scale * score.kGrad;
     const int64_t to = (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, row_q = (int64_t)p.hq * p.d;
     const auto value = [&](int db, int r) { return acc[db][r] * unscale; };

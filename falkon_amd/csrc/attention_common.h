@@ -262,6 +262,12 @@ template <typename T, int DP, int TR> struct Feed {
 #pragma unroll
         for (int n = 0; n < N; n++) clean<T>(tile + (n * kAttnThreads + threadIdx.x) * 16);
     }
+    // 32 rows of a tile (the rows of a block of products), by all of the workgroup's threads, once they have been read as they came
+    static __device__ __forceinline__ void clean_block(char *tile, int block) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * NC; i += kAttnThreads) clean<T>(tile + (block * 32 * NC + i) * 16);
+        __syncthreads();
+    }
     // whether this thread's share of a tile in LDS holds an infinity or a NaN
     static __device__ __forceinline__ bool nonfinite(const char *tile) {
         unsigned bits = 0;
@@ -411,6 +417,46 @@ __device__ __noinline__ void spread_nonfinite(const T *rows, int64_t stride, int
             }
     }
 }
+
+// Columns of a gradient that are NaN because a value which is not finite stands in them, in a row of the other operand that this row
+// sees: its weight is zero whenever it is finite itself.  A product with such values would reach the rows that hide them too, so it
+// runs on zeros in their place (clean_block) and the columns are kept here, as bits in LDS: 32 rows of a wave, whose lanes of the first half
+// write their own row's bits.
+template <int DP> struct Spoilt {
+    unsigned row[DP / 32];
+    __device__ __forceinline__ void clear() {
+        if ((threadIdx.x & 63) < 32) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) row[i] = 0;
+        }
+    }
+    // the first `n` rows of a tile of the other operand, in memory
+    template <typename T> __device__ __forceinline__ void note(const T *rows, int64_t stride, int n, int d, const Seen &seen) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll 1
+        for (int place = 0; place < n; place++) {
+            const bool mine = lane < 32 && ((place < 32 ? seen.w[0] : seen.w[1]) >> (place & 31) & 1);   // (not shifted in this half)
+#pragma unroll 1
+            for (int c0 = 0; c0 < d; c0 += 64) {
+                const int c = c0 + lane;
+                const uint64_t bad = __ballot(c < d && !(__builtin_fabsf((float)rows[place * stride + min(c, d - 1)]) < kInf));
+                if (bad == 0 || !mine) continue;
+                row[c0 / 32] |= (unsigned)bad;
+                if (c0 + 32 < DP) row[c0 / 32 + 1] |= (unsigned)(bad >> 32);
+            }
+        }
+    }
+    // `x`, the sums of this lane's row
+    __device__ __forceinline__ void mark(fx16 *x) const {
+        const int half = threadIdx.x >> 5 & 1;
+#pragma unroll
+        for (int db = 0; db < DP / 32; db++) {
+            const unsigned w = row[db] >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[db][r] = w >> (8 * (r >> 2) + (r & 3)) & 1 ? __builtin_nanf("") : x[db][r];
+        }
+    }
+};
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 __device__ __forceinline__ int wave_min(int x) {

@@ -158,14 +158,11 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                         s[kb][r] = score(s[kb][r], at - (float)(32 * kb + 8 * (r >> 2) + (r & 3)), grad);
                     }
             }
-            const auto look_at = [&]() {
-                uint64_t see = low_bits(last + 1 - k0);
-                if (p.docs != nullptr) see &= same_id(place_id, id);
-                return seen_from(see);
-            };
             Seen seen = {{~0u, ~0u}};
             if (!full) {
-                seen = look_at();
+                uint64_t see = low_bits(last + 1 - k0);
+                if (p.docs != nullptr) see &= same_id(place_id, id);
+                seen = seen_from(see);
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll

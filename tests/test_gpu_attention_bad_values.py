@@ -48,3 +48,56 @@ def test_an_infinite_value_with_a_weight_of_nothing(dtype):
         assert not bool(out[:, 5:, :, 7].isfinite().any()) and not bool(out[:, 150:, :, 9].isfinite().any())
         out[:, 5:, :, 7], out[:, 150:, :, 9] = 0.0, 0.0
         assert bool(out.isfinite().all())
+
+
+def _infinite_keys(dtype, capped):
+    """Keys with one infinity each, in column 0 or 3, on both sides of the causal masks' tiles.  With a cap their scores are plus or
+    minus the cap, without one minus infinity (the queries' column 0 is +-1 there and column 3 is 1), so every row's sum is finite."""
+    q, k, v, do = _make(1, 300, 300, 2, 2, 64, 64, dtype, seed=32)
+    q[..., 0], q[..., 3] = 1.0, 1.0
+    if capped:
+        q[:, ::3, :, 0] = -1.0
+    bad = [(1, 0, -1), (70, 3, -1), (150, 0, -1), (280, 3, -1)] + ([(40, 0, 1), (200, 3, 1)] if capped else [])
+    for key, c, sign in bad:
+        k[:, key, :, c] = sign * float("inf")
+    return q, k, v, do, bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("capped", [False, True])
+@pytest.mark.parametrize("mask", ["causal", "none", "documents", "prefix"])
+def test_gradients_of_rows_that_see_infinite_keys(dtype, capped, mask):
+    """A capped score's derivative is zero where the score is infinite, and a weight is zero where it is minus infinity: dq and the slopes'
+    gradient are those of a key far out (whose score is as good as infinite), and NaN in the infinity's own column (zero times it)."""
+    q, k, v, do, bad = _infinite_keys(dtype, capped)
+    far = k.clone()
+    for key, c, sign in bad:
+        far[:, key, :, c] = sign * 3e4                                       # a score of 6e3: the cap is reached, or exp(-6e3) = 0
+    slopes = torch.tensor([0.02, 0.0], device=DEV).requires_grad_()
+    kw = dict(causal=mask != "none", scale=0.2, softcap=2.0 if capped else 0.0)
+    if mask == "documents":
+        kw["documents"] = (torch.arange(300, device=DEV) // 130)[None].contiguous()
+    if mask == "prefix":
+        kw["prefix"] = torch.tensor([90], device=DEV)
+    pos = torch.arange(300, device=DEV)
+    see = torch.ones(300, 300, dtype=torch.bool, device=DEV) if mask == "none" else pos[:, None] >= pos[None]
+    if mask == "prefix":
+        see = see | (pos[None] < 90)
+    if mask == "documents":
+        see = see & (kw["documents"][0][:, None] == kw["documents"][0][None])
+
+    def run(keys, sl):
+        leaves = [t.detach().requires_grad_() for t in (q, keys, v)] + ([sl] if sl is not None else [])
+        out = attention(*leaves[:3], slopes=sl, **kw)
+        return out.detach(), torch.autograd.grad(out, leaves, do)
+    for sl in (slopes, None):
+        out, got = run(k, sl)
+        out2, want = run(far, sl)
+        assert torch.equal(out, out2)
+        hit = torch.zeros(1, 300, 2, 64, dtype=torch.bool, device=DEV)
+        for key, c, _ in bad:
+            hit[:, see[:, key], :, c] = True
+        assert bool(got[0][hit].isnan().all())
+        assert torch.equal(got[0][~hit], want[0][~hit])
+        assert sl is None or torch.equal(got[3], want[3])
