@@ -334,21 +334,23 @@ template <typename T, int MOD> struct Score {
         slope = slope_ * kScoreUnit;
     }
     __device__ __forceinline__ float r(float s) const { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * in)); }
-    // x of an inner product s at distance `dist`; `grad` gets the derivative by scale * s, a quarter of it for 16-bit data
+    // x of an inner product s at distance `dist`; `grad` gets the derivative by scale * s, a quarter of it for 16-bit data.  It lies
+    // in [0, 1], also where s is NaN: the masks of the backward pass come before it, and zero times NaN would undo them.  (That is
+    // the clamp of the instruction which forms it and costs nothing; the masks behind it took 2 % of a step with capped scores.)
     __device__ __forceinline__ float operator()(float s, float dist, float &grad) const {
         float x;
         if constexpr (!kHasCap) x = s * unit;
         else if constexpr (!kWide) {
             const float a = r(s);
             x = __builtin_fmaf(a, -2.f * out, out);
-            grad = __builtin_fmaf(-a, a, a);
+            grad = __builtin_amdgcn_fmed3f(__builtin_fmaf(-a, a, a), 0.f, 1.f);
         } else {
             const float u = s * in, w = u * u;
             const float e = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kScoreUnit * u));
             const float near = u * (1.f + w * (-1.f / 3 + w * (2.f / 15 + w * (-17.f / 315 + w * (62.f / 2835)))));
             const float t = __builtin_fabsf(u) < 0.25f ? near : 1.f - 2.f * e;
             x = t * out;
-            grad = 1.f - t * t;
+            grad = __builtin_amdgcn_fmed3f(__builtin_fmaf(-t, t, 1.f), 0.f, 1.f);
         }
         if constexpr (kHasDecay) x = __builtin_fmaf(-slope, __builtin_fabsf(dist), x);
         return x;

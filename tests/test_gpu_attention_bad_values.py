@@ -101,3 +101,23 @@ def test_gradients_of_rows_that_see_infinite_keys(dtype, capped, mask):
         assert bool(got[0][hit].isnan().all())
         assert torch.equal(got[0][~hit], want[0][~hit])
         assert sl is None or torch.equal(got[3], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("decay", [False, True])
+def test_hidden_bad_keys_with_a_cap(dtype, decay):
+    """A hidden score of NaN has a cap's derivative of NaN: it is hidden too."""
+    q, k, v, do = _make(1, 200, 200, 2, 2, 64, 64, dtype, seed=36)
+    ids = (torch.arange(200, device=DEV) // 70)[None].contiguous()
+    ids[:, 180:] = -1
+    slopes = torch.tensor([0.1, 0.01], device=DEV).requires_grad_() if decay else None
+
+    def run(k, v):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)] + ([slopes] if decay else [])
+        return torch.autograd.grad(attention(*leaves[:3], slopes=slopes, causal=True, documents=ids, softcap=3.0), leaves, do)
+    want = run(k, v)
+    for value in (float("nan"), float("inf")):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, 185, :, 9], v2[:, 190, :, 3] = value, value
+        assert all(torch.equal(a, b) for a, b in zip(run(k2, v2), want))
