@@ -8,6 +8,9 @@
 // Two kernels instead of one with atomic sums of dq: seven products instead of five, and gradients that are the same run to
 // run.  The first owns queries (dq, the rows' statistics, the slopes' partial sums), the second keys (dk, dv; it walks over
 // the query heads that share its key head, so those are summed in registers).
+//
+// Infinities and NaNs reach what sees them as in these formulas, in tiles with a mask and without: a matrix product would carry them to
+// what does not, so they never enter one whose other operand has hidden places.
 #include "attention_common.h"
 
 namespace flk {
@@ -64,8 +67,6 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
 #pragma unroll
         for (int i = 0; i < AT::E; i++) delta += (float)g.f[i] * ((float)o.f[i] + (float)e.f[i]);
     }
-    // a row with a NaN or an infinity in q or dout has gradients of NaN, and its delta says so to the other kernel
-    if (any_bad<T>(bits)) delta = __builtin_nanf("");
     delta += other_half(delta);
     // the statistics of this tile's rows, for both kernels; a row that sees nothing, or is none, has every p zero
     float lse = kInf;
@@ -73,11 +74,16 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         const float x = p.lse[((int64_t)b * p.hq + h) * p.sq + row];
         lse = x == -kInf ? kInf : x * kScoreUnit;
     }
+    bool bad_row = any_bad<T>(bits);
+    bad_row |= __shfl_xor((int)bad_row, 32, 64) != 0;
     if (half == 0 && part == 0) {
-        float *st = p.stats + ((int64_t)b * p.hq + h) * 2 * p.sq_pad + row;
-        st[0] = lse;
+        float *st = p.stats + ((int64_t)b * p.hq + h) * 3 * p.sq_pad + row;
+        st[0] = bad_row ? kInf : lse;
         st[p.sq_pad] = delta;
+        st[2 * p.sq_pad] = lse;
     }
+    const int bad_wave = (__any(bad_row) ? 1 : 0) | (__any(bad_row && lse != kInf) ? 2 : 0);
+    if (lane == 0 && part == 0) p.bad_rows[(((int64_t)b * p.hq + h) * p.sq_pad + i0) / 32 + wave] = (unsigned char)bad_wave;
 
     int id = 0;
     int2 span = {0, 0}, wg_span = {0, 0};
@@ -283,6 +289,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ __align__(16) float lds_stat[2][2][TQ];             // lse and delta of a tile's rows
     __shared__ int lds_doc[8];
+    __shared__ int lds_bad[4];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int pairs = p.b * p.hk, tiles_k = (p.sk + kAttnRows - 1) / kAttnRows;
@@ -295,6 +302,25 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int prefix = p.prefix != nullptr ? max(min(p.prefix[b], p.sk), 0) : 0;
     const int first = p.causal && key >= prefix ? key - off : 0;   // first row that sees this key
 
+    // rows that may see a key of this tile: with the causal mask those at or behind its first key, or all for a prefix.
+    // (A row past the last one is masked like a hidden one: zero times an infinity of a key would be its score.)
+    const int lo = p.causal && k0 >= prefix ? max(k0 - off, 0) : 0;
+    const int tile_lo = lo / TQ, tile_end = (p.sq + TQ - 1) / TQ;
+    const int64_t tiles_q = max(0, tile_end - tile_lo);
+    const int walk_lo = tile_lo + (int)(tiles_q * row_part / p.row_parts), walk_end = tile_lo + (int)(tiles_q * (row_part + 1) / p.row_parts);
+    // the heads that share this key head, one after the other; the tiles to visit are the same for each
+    int head = p.group * head_part / p.head_parts;                 // of the tile on its way
+    const int head_end = p.group * (head_part + 1) / p.head_parts;
+    // Whether any of the rows that this workgroup goes over is not finite.  (Asked for first, so that the answer is on its way together
+    // with keys and values.)
+    bool bad = false;
+    {
+        const int n = (walk_end * TQ + kAttnRows - 1) / kAttnRows - walk_lo * TQ / kAttnRows, all = n * (head_end - head);
+        for (int i = threadIdx.x; i < all; i += kAttnThreads) {
+            const int64_t of = (int64_t)b * p.hq + hk * p.group + head + i / n;
+            bad |= ((const int *)p.bad_rows)[of * (p.sq_pad / kAttnRows) + walk_lo * TQ / kAttnRows + i % n] != 0;
+        }
+    }
     const T *krow = (const T *)p.k + b * p.ks.b + hk * p.ks.h + (int64_t)key * p.ks.s;
     const T *vrow = (const T *)p.v + b * p.vs.b + hk * p.vs.h + (int64_t)key * p.vs.s;
     typename TL::Lane at_lane;
@@ -312,22 +338,25 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     int2 span = {0, 0}, wg_span = {0, 0};
     const int2 *ranges = p.doc_range + (int64_t)b * p.doc_blocks;
     const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
+    const bool bad_wave = __any(bad);
+    if (lane == 0) lds_bad[wave] = bad_wave;
     if (p.docs != nullptr) {
         const int raw = live ? ids[key] : -1;
         span = {wave_min(raw), wave_max(raw)};
         if (lane == 0) { lds_doc[wave] = span.x; lds_doc[4 + wave] = span.y; }
         id = raw;
-        __syncthreads();
+    }
+    __syncthreads();
+    bad = (lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3]) != 0;
+    if (p.docs != nullptr) {
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
     }
-    // rows that may see a key of this tile: with the causal mask those at or behind its first key, or all for a prefix.
-    // A row past the last one has statistics that make its weights zero, and needs no mask.
-    const int lo = p.causal && k0 >= prefix ? max(k0 - off, 0) : 0;
     const auto look = [&](int t, bool &want, bool &whole, bool &full, bool &skip) {
         const int i0 = t * TQ, i1 = min(i0 + TQ, p.sq);
-        whole = !p.causal || k0 + kAttnRows - 1 <= i0 + off || k0 + kAttnRows <= prefix;
-        full = !p.causal || k_lo + 31 <= i0 + off || k_lo + 32 <= prefix;
+        const bool inside = i0 + TQ <= p.sq;
+        whole = inside && (!p.causal || k0 + kAttnRows - 1 <= i0 + off || k0 + kAttnRows <= prefix);
+        full = inside && (!p.causal || k_lo + 31 <= i0 + off || k_lo + 32 <= prefix);
         skip = p.causal && k_lo > i0 + TQ - 1 + off && k_lo >= prefix;
         if (p.docs != nullptr) {
             const int2 s = doc_span(ranges, i0 + off, i1 + off);
@@ -342,14 +371,11 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
 #pragma unroll
     for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
 
-    // the heads that share this key head, one after the other; the tiles to visit are the same for each
-    int head = p.group * head_part / p.head_parts;                 // of the tile on its way
-    const int head_end = p.group * (head_part + 1) / p.head_parts;
     Score<T, MOD> score(p.scale, p.cap, 0.f);
     FD feed_q, feed_g;
     feed_q.init((const T *)p.q + b * p.qs.b + (hk * p.group + head) * p.qs.h, p.qs.s, p.d, p.vec);
     feed_g.init((const T *)p.dout + b * p.dos.b + (hk * p.group + head) * p.dos.h, p.dos.s, p.dv_d, p.vec_v);
-    const float *stats = p.stats + ((int64_t)b * p.hq + hk * p.group + head) * 2 * p.sq_pad;
+    const float *stats = p.stats + ((int64_t)b * p.hq + hk * p.group + head) * 3 * p.sq_pad;
     // a tile's statistics (padded to whole tiles of 128 rows) pass through registers of its first threads
     float r_lse = 0.f, r_delta = 0.f;
     int place_id = -1, next_id = -1;                               // id of row i0 + lane, one tile ahead
@@ -367,10 +393,8 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const auto put = [&](int to) {
         if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; }
     };
-    const int tile_lo = lo / TQ, tile_end = (p.sq + TQ - 1) / TQ;
     TileWalk walk, again;
-    const int64_t tiles_q = max(0, tile_end - tile_lo);
-    walk.start(tile_lo + (int)(tiles_q * row_part / p.row_parts), tile_lo + (int)(tiles_q * (row_part + 1) / p.row_parts));
+    walk.start(walk_lo, walk_end);
     int tile = walk.next(look);
     again = walk;                                                  // the first 64 tiles as they were found
     const int first_tile = tile;
@@ -381,7 +405,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
         head++;
         feed_q.base += p.qs.h;
         feed_g.base += p.dos.h;
-        stats += 2 * p.sq_pad;
+        stats += 3 * p.sq_pad;
         walk = again;
         walk.is_whole = first_whole;
         walk.is_full = first_full;
@@ -407,17 +431,15 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
             __syncthreads();
             buf ^= 1;
             if (next >= 0) issue(next, lds + buf * 2 * kTileBytes);
-            if (!whole && __any(!(__builtin_fabsf(delta_of[lane % TQ]) < kInf))) {   // a row that is not finite, hidden from some keys
+            if (bad) {                                             // rows that are not finite, which attention_bad_rows_kernel adds
                 FD::clean_share(lds_q);
                 FD::clean_share(lds_g);
-                // keys that do see it get weights of NaN for it
-                if (mine && !(__builtin_fabsf(delta_of[threadIdx.x]) < kInf)) lds_stat[buf ^ 1][0][threadIdx.x] = __builtin_nanf("");
                 __syncthreads();
             }
             if (!skip) {
                 Seen seen = {{~0u, ~0u}};
                 if (!full) {
-                    uint64_t see = ~low_bits(first - i0);
+                    uint64_t see = low_bits(p.sq - i0) & ~low_bits(first - i0);
                     if (p.docs != nullptr) see &= same_id(place_id, id);
                     seen = seen_from(see);
                 }
@@ -558,6 +580,126 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     }
 }
 
+// What rows of q and dout with infinities or NaNs, which have no weight in the kernel above, do to dk and dv of the keys that see
+// them: one row after the other, by vector instructions, added to what was written (to the first of its parts).  A product of matrices
+// would carry their NaNs (zero times an infinity) to the keys that do not see them.  A workgroup goes over the rows for 128 keys, and has
+// nothing to do where all rows are finite (3 us; as a branch of the kernel above it took 5 % of its time by its registers).
+template <typename T, int DP, int MOD>
+__global__ void __launch_bounds__(kAttnThreads) attention_bad_rows_kernel(AttnArgs p) {
+    typedef AttnType<T> AT;
+    typedef typename AT::frag frag;
+    constexpr int C = DP / AT::KS, DB = DP / 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int pairs = p.b * p.hk, pair = blockIdx.x % pairs, tile_k = blockIdx.x / pairs, b = pair / p.hk, hk = pair % p.hk;
+    const int off = p.sk - p.sq, k_lo = tile_k * kAttnRows + wave * 32, key = k_lo + (lane & 31);
+    const bool live = key < p.sk;
+    const int64_t flags = p.sq_pad / 32, line0 = (int64_t)b * p.hq + hk * p.group;
+    // (a key head's flags lie one after the other)
+    bool bad = false;
+    for (int64_t i = lane; i < flags * p.group / 4; i += 64) bad |= (((const int *)p.bad_rows)[line0 * flags / 4 + i] & 0x02020202) != 0;
+    if (!__any(bad)) return;
+    const int prefix = p.prefix != nullptr ? max(min(p.prefix[b], p.sk), 0) : 0;
+    const int first = p.causal && key >= prefix ? key - off : 0;   // first row that sees this key
+    const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
+    const int id = p.docs != nullptr && live ? ids[key] : 0;
+    const T *krow = (const T *)p.k + b * p.ks.b + hk * p.ks.h + (int64_t)key * p.ks.s;
+    const T *vrow = (const T *)p.v + b * p.vs.b + hk * p.vs.h + (int64_t)key * p.vs.s;
+    frag kf[C], vf[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        union { ux4 u; frag f; } x, y;
+        x.u = load_chunk<T>(krow, 2 * c + half, p.d, live, p.vec);
+        y.u = load_chunk<T>(vrow, 2 * c + half, p.dv_d, live, p.vec_v);
+        kf[c] = x.f;
+        vf[c] = y.f;
+    }
+    fx16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++) dk[db] = dv[db] = fx16{};
+    bool all_nan = false;
+    for (int g = 0; g < p.group; g++) {
+        const int h = hk * p.group + g;
+        const T *q0 = (const T *)p.q + b * p.qs.b + h * p.qs.h;
+        const T *g0 = (const T *)p.dout + b * p.dos.b + h * p.dos.h;
+        const Score<T, MOD> score(p.scale, p.cap, (MOD & kDecay) && p.slopes != nullptr ? p.slopes[h] : 0.f);
+        const float *lse_of = p.stats + (line0 + g) * 3 * p.sq_pad, *delta_of = lse_of + p.sq_pad, *true_lse_of = delta_of + p.sq_pad;
+        uint64_t todo = 0;
+        int i0 = (p.causal && k_lo >= prefix ? max(k_lo - off, 0) : 0) / 32 * 32 - 32;
+#pragma unroll 1
+        while (!all_nan) {                                         // (which is what they soon are where no row is finite)
+            while (todo == 0 && (i0 += 32) < p.sq) {
+                if (!(p.bad_rows[(line0 + g) * flags + i0 / 32] & 2)) continue;
+                const int at = i0 + (lane & 31);
+                todo = (uint32_t)__ballot(lse_of[at] == kInf && true_lse_of[at] != kInf);
+            }
+            if (todo == 0) break;
+            const int i = i0 + __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const float lse = true_lse_of[i], delta = delta_of[i];
+            const bool see = live && i >= first && (p.docs == nullptr || (id >= 0 && ids[i + off] == id));
+            if (!__any(see)) continue;
+            const T *qi = q0 + i * p.qs.s, *gi = g0 + i * p.dos.s;
+            float s = 0.f, dp = 0.f, grad = 1.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                union { ux4 u; frag f; } x, y;
+                x.u = load_chunk<T>(qi, 2 * c + half, p.d, true, p.vec);
+                y.u = load_chunk<T>(gi, 2 * c + half, p.dv_d, true, p.vec_v);
+#pragma unroll
+                for (int j = 0; j < AT::E; j++) { s += (float)x.f[j] * (float)kf[c][j]; dp += (float)y.f[j] * (float)vf[c][j]; }
+            }
+            s += other_half(s);
+            dp += other_half(dp);
+            const float e = __builtin_amdgcn_exp2f(score(s, (float)(i + off - key), grad) - lse);
+            float x = dp - delta;
+            if constexpr ((MOD & kCap) != 0) x *= grad;
+            const float ds = times_or_zero(e, x);
+            int c0 = 4 * half;
+            asm volatile("" : "+v"(c0));                           // (or the comparisons below are made ahead and kept)
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int c = c0 + 32 * db + 8 * (r >> 2) + (r & 3);
+                    const float qc = c < p.d ? (float)qi[c] : 0.f, gc = c < p.dv_d ? (float)gi[c] : 0.f;
+                    if (see) {
+                        dk[db][r] += ds * qc;
+                        dv[db][r] += __builtin_fabsf(gc) < kInf ? e * gc : __builtin_nanf("");
+                    }
+                }
+            bool nan = true;
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int c = c0 + 32 * db + 8 * (r >> 2) + (r & 3);
+                    nan &= (c >= p.d || dk[db][r] != dk[db][r]) && (c >= p.dv_d || dv[db][r] != dv[db][r]);
+                }
+            all_nan = !__any(live && !nan);
+        }
+    }
+    if (!live) return;
+    const int splits = p.head_parts * p.row_parts;
+    const int64_t keys = (int64_t)p.b * p.sk * p.hk, row = ((int64_t)b * p.sk + key) * p.hk + hk;
+    const float unscale = p.scale * Score<T, MOD>::kGrad;
+    const auto add = [&](auto *to, const fx16 *x, int n, float by) {
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int c = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
+                if (c < n) to[c] = (std::remove_reference_t<decltype(*to)>)((float)to[c] + x[db][r] * by);
+            }
+    };
+    if (splits == 1) {
+        add((T *)p.dk + row * p.d, dk, p.d, unscale);
+        add((T *)p.dv + row * p.dv_d, dv, p.dv_d, 1.f);
+    } else {
+        add(p.dkv_part + row * p.d, dk, p.d, unscale);
+        add(p.dkv_part + splits * keys * p.d + row * p.dv_d, dv, p.dv_d, 1.f);
+    }
+}
+
 template <typename T> int launch_attention_dq(const AttnArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hq * ((a.sq + kAttnRows - 1) / kAttnRows) * a.parts));
     FLK_ATTN_LAUNCH(attention_dq_kernel, grid)
@@ -566,6 +708,8 @@ template <typename T> int launch_attention_dq(const AttnArgs &a, int dp, hipStre
 template <typename T> int launch_attention_dkv(const AttnArgs &a, int dp, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.head_parts * a.row_parts * ((a.sk + kAttnRows - 1) / kAttnRows)));
     FLK_ATTN_LAUNCH(attention_dkv_kernel, grid)
+    const dim3 tiles((unsigned)((int64_t)a.b * a.hk * ((a.sk + kAttnRows - 1) / kAttnRows)));
+    if (a.sq > 0) FLK_ATTN_LAUNCH_KIND(attention_bad_rows_kernel, tiles)
     return FLK_OK;
 }
 template int launch_attention_dq<attn_t>(const AttnArgs &, int, hipStream_t);

@@ -157,7 +157,10 @@ struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
     void *o, *rest, *dq, *dk, *dv;                     // rest: what rounding took from out, for the backward pass
     float *lse, *dslopes_part, *dq_part, *dkv_part;
-    float *stats;                                      // backward: [b][hq][2][sq_pad], the rows' lse (in units of log 2) and delta
+    // backward: [b][hq][3][sq_pad], the rows' lse (in units of log 2; infinite, so that weights are zero, for a row of q or dout that holds
+    // infinities or NaNs), delta, and the lse without that
+    float *stats;
+    unsigned char *bad_rows;                           // backward: [b][hq][sq_pad / 32], whether there is such a row among 32 (1) that sees something (2)
     int64_t sq_pad;
     AttnStride qs, ks, vs, dos;                        // strides of q, k, v and dout; the others are contiguous
     int b, sq, sk, hq, hk, group, d, dv_d;
@@ -540,13 +543,17 @@ inline int score_kind(float scale, float cap, const float *slopes) {
         else if (kind == kDecay) hipLaunchKernelGGL((KERNEL<T, DP, kDecay>), GRID, dim3(kAttnThreads), 0, st, a);  \
         else hipLaunchKernelGGL((KERNEL<T, DP, kCapDecay>), GRID, dim3(kAttnThreads), 0, st, a);                   \
     }
+#define FLK_ATTN_LAUNCH_KIND(KERNEL, GRID)                         \
+    {                                                              \
+        if (dp == 32) FLK_ATTN_KIND(KERNEL, 32, GRID)              \
+        else if (dp == 64) FLK_ATTN_KIND(KERNEL, 64, GRID)         \
+        else if (dp == 96) FLK_ATTN_KIND(KERNEL, 96, GRID)         \
+        else FLK_ATTN_KIND(KERNEL, 128, GRID)                      \
+        FLK_LAUNCH_CHECK(#KERNEL);                                 \
+    }
 #define FLK_ATTN_LAUNCH(KERNEL, GRID)                              \
     const int kind = score_kind(a.scale, a.cap, a.slopes);         \
-    if (dp == 32) FLK_ATTN_KIND(KERNEL, 32, GRID)                  \
-    else if (dp == 64) FLK_ATTN_KIND(KERNEL, 64, GRID)             \
-    else if (dp == 96) FLK_ATTN_KIND(KERNEL, 96, GRID)             \
-    else FLK_ATTN_KIND(KERNEL, 128, GRID)                          \
-    FLK_LAUNCH_CHECK(#KERNEL);
+    FLK_ATTN_LAUNCH_KIND(KERNEL, GRID)
 
 #if defined(FLK_KF)
 #if FLK_KF == 0

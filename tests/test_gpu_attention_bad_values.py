@@ -105,6 +105,110 @@ def test_gradients_of_rows_that_see_infinite_keys(dtype, capped, mask):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("capped", [False, True])
+@pytest.mark.parametrize("sq", [300, 320, 33])
+def test_gradients_of_infinite_keys(dtype, capped, sq):
+    """dk and dv of every key, the infinite ones among them, are those of keys far out; also where a tile holds rows past the last
+    one, whose queries are zero, and zero times an infinity is their score."""
+    q, k, v, do, bad = _infinite_keys(dtype, capped)
+    q, do = q[:, -sq:], do[:, -sq:]
+    far = k.clone()
+    for key, c, sign in bad:
+        far[:, key, :, c] = sign * 3e4
+    for causal in (False, True):
+        got, want = ([t for t in _grads(q, keys, v, do, causal=causal and sq <= 300, scale=0.2, softcap=2.0 if capped else 0.0)] for keys in (k, far))
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2]) and bool(want[1].isfinite().all())
+
+
+def _within(got, want, where):
+    """Inside the bounds of ``attention_ref`` at these places.  (A row that is not finite is added to dk and dv by itself, behind the
+    others and with unrounded weights, so they are not the same to the last bit.)"""
+    value, bound = want
+    off = (got.double().cpu() - value).abs()[where.cpu()]
+    assert bool((off <= bound[where.cpu()]).all())
+
+
+def _grads(q, k, v, do, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    return torch.autograd.grad(attention(*leaves, **kw), leaves, do)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("mask", ["causal", "none", "documents"])
+def test_dv_does_not_depend_on_v(dtype, d, mask):
+    """dv is the weights' transpose times dout: NaNs and infinities of v that rows see are in out, dq and dk, and not in dv."""
+    q, k, v, do = _make(1, 290, 290, 4, 2, d, d, dtype, seed=33)
+    kw = dict(causal=mask != "none")
+    if mask == "documents":
+        kw["documents"] = (torch.arange(290, device=DEV) // 100)[None].contiguous()
+    want = _grads(q, k, v, do, **kw)
+    v2 = v.clone()
+    v2[:, 130, :, 1], v2[:, 285, :, d - 1] = float("nan"), -float("inf")
+    got = _grads(q, k, v2, do, **kw)
+    assert torch.equal(got[2], want[2])
+    assert not bool(got[0][:, 285:].isfinite().any())
+    if mask == "causal":
+        assert torch.equal(got[0][:, :130], want[0][:, :130]) and not bool(got[1][:, :286].isfinite().any())
+        assert torch.equal(got[1][:, 286:].isfinite(), torch.zeros_like(got[1][:, 286:], dtype=torch.bool))
+    if mask == "documents":                                                  # documents 0 .. 99, 100 .. 199, 200 .. 289
+        assert torch.equal(got[0][:, :130], want[0][:, :130]) and torch.equal(got[0][:, 200:285], want[0][:, 200:285])
+        assert torch.equal(got[1][:, :100], want[1][:, :100]) and not bool(got[1][:, 200:286].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("mask", ["causal", "none", "documents"])
+def test_gradients_of_keys_that_see_one_bad_value_of_dout(dtype, d, mask):
+    """dv is not finite in that column and dk nowhere; dv's other columns and the other keys are as they were."""
+    q, k, v, do = _make(1, 290, 290, 4, 2, d, d, dtype, seed=34)
+    kw = dict(causal=mask != "none")
+    if mask == "documents":
+        kw["documents"] = (torch.arange(290, device=DEV) // 100)[None].contiguous()
+    want, exact = _grads(q, k, v, do, **kw), reference(q, k, v, do, **kw)
+    for value in (float("nan"), float("inf")):
+        do2 = do.clone()
+        do2[:, 150, 1, 5] = value                                            # a head that shares key head 0
+        got = _grads(q, k, v, do2, **kw)
+        lo, hi = {"causal": (0, 151), "none": (0, 290), "documents": (100, 151)}[mask]
+        hit = torch.zeros(1, 290, 2, d, dtype=torch.bool, device=DEV)
+        hit[:, lo:hi, 0, 5] = True
+        assert not bool(got[2][hit].isfinite().any())
+        _within(got[2], exact["dv"], ~hit)
+        assert torch.equal(got[2][:, :lo], want[2][:, :lo]) and torch.equal(got[2][:, hi:], want[2][:, hi:]) and torch.equal(got[2][:, :, 1], want[2][:, :, 1])
+        assert not bool(got[1][:, lo:hi, 0].isfinite().any())
+        assert torch.equal(got[1][:, :lo], want[1][:, :lo]) and torch.equal(got[1][:, hi:], want[1][:, hi:]) and torch.equal(got[1][:, :, 1], want[1][:, :, 1])
+        row = torch.zeros(1, 290, 4, d, dtype=torch.bool, device=DEV)
+        row[:, 150, 1] = True
+        assert torch.equal(got[0][~row], want[0][~row]) and not bool(got[0][row].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", ["causal", "none"])
+def test_gradients_of_rows_with_an_infinity_and_a_cap(dtype, mask):
+    """Such a row's scores are plus or minus the cap and have no gradient: dv and dq are those of a row far out, dk is NaN in the
+    infinity's own column (zero times it) for the keys that the row sees, and elsewhere that of a row far out."""
+    q, k, v, do = _make(1, 290, 290, 2, 2, 64, 64, dtype, seed=35)
+    k[..., 2] = torch.where(k[..., 2] < 0, -1.0, 1.0).to(dtype)
+    far, q2 = q.clone(), q.clone()
+    far[:, 140, :, 2], q2[:, 140, :, 2] = 3e4, float("inf")
+    kw = dict(causal=mask == "causal", scale=0.2, softcap=2.0)
+    got, want = _grads(q2, k, v, do, **kw), _grads(far, k, v, do, **kw)
+    hit = torch.zeros(1, 290, 2, 64, dtype=torch.bool, device=DEV)
+    hit[:, :141 if mask == "causal" else 290, :, 2] = True
+    assert torch.equal(got[0], want[0]) and bool(got[1][hit].isnan().all())
+    exact = reference(far, k, v, do, **kw)
+    _within(got[1], exact["dk"], ~hit)
+    _within(got[2], exact["dv"], torch.ones_like(hit))
+    if mask == "causal":
+        assert torch.equal(got[1][:, 141:], want[1][:, 141:]) and torch.equal(got[2][:, 141:], want[2][:, 141:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("decay", [False, True])
 def test_hidden_bad_keys_with_a_cap(dtype, decay):
     """A hidden score of NaN has a cap's derivative of NaN: it is hidden too."""
@@ -121,3 +225,19 @@ def test_hidden_bad_keys_with_a_cap(dtype, decay):
         k2, v2 = k.clone(), v.clone()
         k2[:, 185, :, 9], v2[:, 190, :, 3] = value, value
         assert all(torch.equal(a, b) for a, b in zip(run(k2, v2), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_where_nothing_is_finite(dtype):
+    q, k, v, do = _make(1, 700, 700, 4, 2, 64, 64, dtype, seed=37)
+    nan = torch.full_like(q, float("nan"))
+    for kw in (dict(), dict(causal=True)):
+        for rows, douts in ((nan, do), (q, nan)):
+            got = _grads(rows, k, v, douts, **kw)
+            assert all(bool(t.isnan().all()) for t in got[:2]) and bool(got[2].isnan().all())
+    ids = torch.zeros(1, 700, dtype=torch.int32, device=DEV)
+    ids[:, 200:600] = -1                                                     # padding between, which holds nothing else
+    want = _grads(q, k, v, do, causal=True, documents=ids)
+    q[:, 200:600], do[:, 250:600] = float("nan"), float("inf")
+    assert all(torch.equal(a, b) for a, b in zip(_grads(q, k, v, do, causal=True, documents=ids), want))
