@@ -390,7 +390,7 @@ template <typename T, int VEC> void norm_forward(const NormArgs<T> &a, const Nor
 template <typename T, int VEC> void norm_backward(const NormArgs<T> &a, const NormPlan &plan, int64_t groups, hipStream_t st) {
 #define FLK_CALL(TPR, NV)                                                                                              \
     if constexpr (NV == 0) {                                                                                           \
-        if (a.y != nullptr)                                                                                            \
+        if (a.y != nullptr && a.rows > 0)                                                                              \
             hipLaunchKernelGGL((layer_norm_bwd_long_kernel<T>), dim3((unsigned)norm_min(a.rows, 4096)), dim3(kLoopThreads), 0, st, a); \
         if (a.partial != nullptr)                                                                                      \
             hipLaunchKernelGGL((layer_norm_columns_kernel<T>), dim3((unsigned)((a.d + kRowThreads - 1) / kRowThreads), (unsigned)groups), \
