@@ -24,7 +24,8 @@ template <> struct NormAcc<double> { typedef double type; };
 __device__ __forceinline__ float rsqrt_of(float x) { return 1.0f / sqrtf(x); }
 __device__ __forceinline__ double rsqrt_of(double x) { return 1.0 / sqrt(x); }
 
-template <typename T, int VEC> struct alignas(VEC * sizeof(T)) NormVec { T v[VEC]; };
+// (16 bytes are what the callers see to: eight float weights beside eight 16-bit values are two such)
+template <typename T, int VEC> struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) NormVec { T v[VEC]; };
 
 // `VEC` consecutive values from element i of a row on, converted; past `d` zero
 template <typename T, int VEC, typename A>
