@@ -6,7 +6,10 @@
 //
 // Both passes move every value once and are bound by memory.  A row lies in the registers of `TPR` threads (NV vectors
 // of 16 bytes each), so mean and centred sum of squares are two passes over registers, not over memory, and nothing
-// cancels as it does in sum(x^2) - mean^2.  Sums are held in 32 bits (64 for double).  Short rows share a wave (28
+// cancels as it does in sum(x^2) - mean^2.  Sums are held in 32 bits (64 for double).  What that leaves in the mean, a few units of its
+// last digit, is the same for all values of a row (a row of 784 times 10000.1 would come out as -0.3): it is the mean of the centred
+// values r, so the second pass sums them too, takes c = sum(r) / d from each and c^2 from the variance.  The backward pass, whose z start
+// from the rounded mean, does the same with the mean of z.  Short rows share a wave (28
 // floats: eight threads a row), rows of more than kRowThreads * 8 vectors are read again instead of being kept.
 // In the backward pass a workgroup walks over many rows and keeps its share of dw and db in registers; it writes one
 // partial row at its end, and a second kernel adds those in a fixed order: no atomics, results are the same run to run.
@@ -71,19 +74,35 @@ __device__ __forceinline__ A row_sum(A x, A *lds) {
     return x;
 }
 
-// Two sums at once; with four waves a row one barrier suffices if the caller alternates between two places in LDS.
-template <int TPR, typename A>
-__device__ __forceinline__ void row_sums(A &x, A &y, A *lds) {
+// N sums at once; with several waves a row one barrier suffices if another stands between this call's reads and the next one's writes
+// (the caller alternates between two places in LDS, or sums something else in between).
+template <int TPR, int N, typename A>
+__device__ __forceinline__ void row_sums(A (&x)[N], A *lds) {
 #pragma unroll
-    for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) { x += __shfl_xor(x, off, 64); y += __shfl_xor(y, off, 64); }
+    for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] += __shfl_xor(x[i], off, 64);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) { lds[2 * wave] = x; lds[2 * wave + 1] = y; }
-        __syncthreads();
-        x = y = A(0);
+        if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int w = 0; w < TPR / 64; w++) { x += lds[2 * w]; y += lds[2 * w + 1]; }
+            for (int i = 0; i < N; i++) lds[N * wave + i] = x[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = A(0);
+#pragma unroll
+            for (int w = 0; w < TPR / 64; w++) x[i] += lds[N * w + i];
+        }
     }
+}
+// The correction c of a rounded mean, and the variance, from the sums of the centred values and of their squares
+template <typename A> __device__ __forceinline__ A centre(const A (&sums)[2], A inv_d, A &var) {
+    const A c = sums[0] * inv_d;
+    var = sums[1] * inv_d - c * c;
+    var = var < A(0) ? A(0) : var;                                 // (NaN stays NaN)
+    return c;
 }
 
 template <typename T> struct NormArgs {
@@ -93,6 +112,7 @@ template <typename T> struct NormArgs {
     const void *w, *b;
     acc *mean, *rstd;
     acc *partial;          // backward: [workgroups][2][d]
+    acc *shift;            // backward, long rows: the mean of z, [rows]
     int64_t rows, d, x_rs, dy_rs;
     int wide;              // w and b are float
     double eps;
@@ -102,7 +122,7 @@ template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(kRowThreads) layer_norm_kernel(NormArgs<T> p) {
     typedef typename NormArgs<T>::acc A;
     constexpr int kRows = kRowThreads / TPR;
-    __shared__ A lds[kRowThreads / 64];
+    __shared__ A lds[3 * kRowThreads / 64];
     const int sub = threadIdx.x % TPR;
     const A inv_d = A(1) / A(p.d);
     for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kRows) {
@@ -118,17 +138,22 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_kernel(NormArgs<T> p) 
             for (int j = 0; j < VEC; j++) s += r[n][j];
         }
         const A mean = row_sum<TPR, A>(s, lds) * inv_d;
-        s = A(0);
+        A sums[2] = {A(0), A(0)}, var;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             if ((int64_t)(n * TPR + sub) * VEC < p.d) {
 #pragma unroll
-                for (int j = 0; j < VEC; j++) { r[n][j] -= mean; s += r[n][j] * r[n][j]; }
+                for (int j = 0; j < VEC; j++) { r[n][j] -= mean; sums[0] += r[n][j]; sums[1] += r[n][j] * r[n][j]; }
             }
         }
-        const A rstd = rsqrt_of(row_sum<TPR, A>(s, lds) * inv_d + A(p.eps));
+        row_sums<TPR, 2, A>(sums, lds + kRowThreads / 64);
+        const A c = centre(sums, inv_d, var), rstd = rsqrt_of(var + A(p.eps));
         if (!live) continue;
-        if (sub == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
+        if (sub == 0 && p.mean != nullptr) { p.mean[row] = mean + c; p.rstd[row] = rstd; }
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) r[n][j] -= c;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             const int64_t i = (int64_t)(n * TPR + sub) * VEC;
@@ -155,22 +180,23 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_kernel(NormArgs<T> p) 
 template <typename T>
 __global__ void __launch_bounds__(kLoopThreads) layer_norm_long_kernel(NormArgs<T> p) {
     typedef typename NormArgs<T>::acc A;
-    __shared__ A lds[kLoopThreads / 64];
+    __shared__ A lds[3 * kLoopThreads / 64];
     const A inv_d = A(1) / A(p.d);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = p.x + row * p.x_rs;
         A s = A(0);
         for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) s += to_acc<A>(x[i]);
         const A mean = row_sum<kLoopThreads, A>(s, lds) * inv_d;
-        s = A(0);
-        for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) { const A c = to_acc<A>(x[i]) - mean; s += c * c; }
-        const A rstd = rsqrt_of(row_sum<kLoopThreads, A>(s, lds) * inv_d + A(p.eps));
-        if (threadIdx.x == 0 && p.mean != nullptr) { p.mean[row] = mean; p.rstd[row] = rstd; }
+        A sums[2] = {A(0), A(0)}, var;
+        for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) { const A r = to_acc<A>(x[i]) - mean; sums[0] += r; sums[1] += r * r; }
+        row_sums<kLoopThreads, 2, A>(sums, lds + kLoopThreads / 64);
+        const A c = centre(sums, inv_d, var), rstd = rsqrt_of(var + A(p.eps));
+        if (threadIdx.x == 0 && p.mean != nullptr) { p.mean[row] = mean + c; p.rstd[row] = rstd; }
         for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) {
             A w = A(1), b = A(0);
             if (p.w != nullptr) load_weight<T, 1, A>(p.w, p.wide, i, p.d, &w);
             if (p.b != nullptr) load_weight<T, 1, A>(p.b, p.wide, i, p.d, &b);
-            p.y[row * p.d + i] = from_acc<T>((to_acc<A>(x[i]) - mean) * (rstd * w) + b);
+            p.y[row * p.d + i] = from_acc<T>((to_acc<A>(x[i]) - mean - c) * (rstd * w) + b);
         }
     }
 }
@@ -180,7 +206,7 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_bwd_kernel(NormArgs<T>
     typedef typename NormArgs<T>::acc A;
     constexpr int kRows = kRowThreads / TPR;
     constexpr int kWidth = TPR * NV * VEC;             // columns a row's threads hold
-    constexpr int kLds = TPR <= 64 ? 2 * kWidth : 4 * (kRowThreads / 64);
+    constexpr int kLds = TPR <= 64 ? 2 * kWidth : 6 * (kRowThreads / 64);
     __shared__ A lds[kLds];
     const int sub = threadIdx.x % TPR;
     const A inv_d = A(1) / A(p.d);
@@ -213,32 +239,44 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_bwd_kernel(NormArgs<T>
         const bool live = row < p.rows;
         const A mean = n_mean, rstd = n_rstd;
         A z[NV][VEC], g[NV][VEC];
-        A s1 = A(0), s2 = A(0);
+        NormVec<T, VEC> dy[NV];
+        A sums[3] = {A(0), A(0), A(0)};                            // of g, g z and z
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             const int64_t i = (int64_t)(n * TPR + sub) * VEC;
+            dy[n] = ny[n];
             A w[VEC];
             if (p.w != nullptr) load_weight<T, VEC, A>(p.w, p.wide, i, p.d, w);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 z[n][j] = i < p.d ? (to_acc<A>(nx[n].v[j]) - mean) * rstd : A(0);
                 g[n][j] = i < p.d ? to_acc<A>(ny[n].v[j]) : A(0);
-                if (live) { dw[n][j] += g[n][j] * z[n][j]; db[n][j] += g[n][j]; }
                 if (p.w != nullptr) g[n][j] *= w[j];
-                s1 += g[n][j];
-                s2 += g[n][j] * z[n][j];
+                sums[0] += g[n][j];
+                sums[1] += g[n][j] * z[n][j];
+                sums[2] += z[n][j];
             }
         }
         if (row0 + step < p.rows) fetch(row0 + step);
-        row_sums<TPR, A>(s1, s2, lds + (TPR > 64 ? turn * 2 * (kRowThreads / 64) : 0));
-        s1 *= inv_d;
-        s2 *= inv_d;
-        if (p.y == nullptr || !live) continue;
+        row_sums<TPR, 3, A>(sums, lds + (TPR > 64 ? turn * 3 * (kRowThreads / 64) : 0));
+        const A c = sums[2] * inv_d, s1 = sums[0] * inv_d, s2 = sums[1] * inv_d - c * s1;
+        if (!live) continue;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
+            const int64_t i = (int64_t)(n * TPR + sub) * VEC;
+            if (i < p.d) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    z[n][j] -= c;
+                    const A t = to_acc<A>(dy[n].v[j]);
+                    dw[n][j] += t * z[n][j];
+                    db[n][j] += t;
+                }
+            }
+            if (p.y == nullptr) continue;
 #pragma unroll
             for (int j = 0; j < VEC; j++) g[n][j] = rstd * (g[n][j] - s1 - z[n][j] * s2);
-            store_vec<T, VEC, A>(p.y + row * p.d, (int64_t)(n * TPR + sub) * VEC, p.d, g[n]);
+            store_vec<T, VEC, A>(p.y + row * p.d, i, p.d, g[n]);
         }
     }
     if (p.partial == nullptr) return;
@@ -284,25 +322,30 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_bwd_kernel(NormArgs<T>
 template <typename T>
 __global__ void __launch_bounds__(kLoopThreads) layer_norm_bwd_long_kernel(NormArgs<T> p) {
     typedef typename NormArgs<T>::acc A;
-    __shared__ A lds[kLoopThreads / 64];
+    __shared__ A lds[2][3 * kLoopThreads / 64];
     const A inv_d = A(1) / A(p.d);
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T *x = p.x + row * p.x_rs, *dy = p.dy + row * p.dy_rs;
         const A mean = p.mean[row], rstd = p.rstd[row];
-        A s1 = A(0), s2 = A(0);
+        A sums[3] = {A(0), A(0), A(0)};                            // of g, g z and z
         for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) {
             A w = A(1);
             if (p.w != nullptr) load_weight<T, 1, A>(p.w, p.wide, i, p.d, &w);
-            const A g = to_acc<A>(dy[i]) * w;
-            s1 += g;
-            s2 += g * ((to_acc<A>(x[i]) - mean) * rstd);
+            const A g = to_acc<A>(dy[i]) * w, z = (to_acc<A>(x[i]) - mean) * rstd;
+            sums[0] += g;
+            sums[1] += g * z;
+            sums[2] += z;
         }
-        s1 = row_sum<kLoopThreads, A>(s1, lds) * inv_d;
-        s2 = row_sum<kLoopThreads, A>(s2, lds) * inv_d;
+        row_sums<kLoopThreads, 3, A>(sums, lds[turn]);
+        const A c = sums[2] * inv_d, s1 = sums[0] * inv_d, s2 = sums[1] * inv_d - c * s1;
+        if (threadIdx.x == 0 && p.shift != nullptr) p.shift[row] = c;
+        if (p.y == nullptr) continue;
         for (int64_t i = threadIdx.x; i < p.d; i += kLoopThreads) {
             A w = A(1);
             if (p.w != nullptr) load_weight<T, 1, A>(p.w, p.wide, i, p.d, &w);
-            p.y[row * p.d + i] = from_acc<T>(rstd * (to_acc<A>(dy[i]) * w - s1 - (to_acc<A>(x[i]) - mean) * rstd * s2));
+            const A z = (to_acc<A>(x[i]) - mean) * rstd - c;
+            p.y[row * p.d + i] = from_acc<T>(rstd * (to_acc<A>(dy[i]) * w - s1 - z * s2));
         }
     }
 }
@@ -310,16 +353,16 @@ __global__ void __launch_bounds__(kLoopThreads) layer_norm_bwd_long_kernel(NormA
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) layer_norm_columns_kernel(NormArgs<T> p) {
     typedef typename NormArgs<T>::acc A;
-    const int64_t c = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-    if (c >= p.d) return;
+    const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+    if (i >= p.d) return;
     A dw = A(0), db = A(0);
     for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
-        const A g = to_acc<A>(p.dy[row * p.dy_rs + c]);
-        dw += g * ((to_acc<A>(p.x[row * p.x_rs + c]) - p.mean[row]) * p.rstd[row]);
+        const A g = to_acc<A>(p.dy[row * p.dy_rs + i]);
+        dw += g * ((to_acc<A>(p.x[row * p.x_rs + i]) - p.mean[row]) * p.rstd[row] - p.shift[row]);
         db += g;
     }
-    p.partial[(int64_t)blockIdx.y * 2 * p.d + c] = dw;
-    p.partial[(int64_t)blockIdx.y * 2 * p.d + p.d + c] = db;
+    p.partial[(int64_t)blockIdx.y * 2 * p.d + i] = dw;
+    p.partial[(int64_t)blockIdx.y * 2 * p.d + p.d + i] = db;
 }
 
 // dw[c] and db[c] from the workgroups' partial rows: 32 columns by 32 slices of the rows a workgroup
@@ -391,7 +434,7 @@ template <typename T, int VEC> void norm_forward(const NormArgs<T> &a, const Nor
 template <typename T, int VEC> void norm_backward(const NormArgs<T> &a, const NormPlan &plan, int64_t groups, hipStream_t st) {
 #define FLK_CALL(TPR, NV)                                                                                              \
     if constexpr (NV == 0) {                                                                                           \
-        if (a.y != nullptr && a.rows > 0)                                                                              \
+        if (a.rows > 0)                                                                                                \
             hipLaunchKernelGGL((layer_norm_bwd_long_kernel<T>), dim3((unsigned)norm_min(a.rows, 4096)), dim3(kLoopThreads), 0, st, a); \
         if (a.partial != nullptr)                                                                                      \
             hipLaunchKernelGGL((layer_norm_columns_kernel<T>), dim3((unsigned)((a.d + kRowThreads - 1) / kRowThreads), (unsigned)groups), \
@@ -419,7 +462,7 @@ static int norm_fwd_impl(const void *x, int64_t rows, int64_t d, int64_t x_rs, c
                          void *y, void *mean, void *rstd, hipStream_t st) {
     const NormPlan plan = norm_plan<T>(d, norm_aligned<T>(d, x, x_rs, nullptr, 0, y, w, b));
     typedef typename NormAcc<T>::type A;
-    NormArgs<T> a{(const T *)x, nullptr, (T *)y, w, b, (A *)mean, (A *)rstd, nullptr, rows, d, x_rs, 0, wide, eps};
+    NormArgs<T> a{(const T *)x, nullptr, (T *)y, w, b, (A *)mean, (A *)rstd, nullptr, nullptr, rows, d, x_rs, 0, wide, eps};
     if (plan.vec == 1) norm_forward<T, 1>(a, plan, st);
     else norm_forward<T, 16 / sizeof(T)>(a, plan, st);
     FLK_LAUNCH_CHECK("layer_norm_kernel");
@@ -428,8 +471,9 @@ static int norm_fwd_impl(const void *x, int64_t rows, int64_t d, int64_t x_rs, c
 
 template <typename T>
 static size_t norm_bwd_bytes(int64_t rows, int64_t d) {        // enough for either row layout
-    const int64_t n = norm_bwd_groups(rows, norm_plan<T>(d, true)), m = norm_bwd_groups(rows, norm_plan<T>(d, false));
-    return (size_t)(n > m ? n : m) * 2 * (size_t)d * sizeof(typename NormAcc<T>::type);
+    const NormPlan plan = norm_plan<T>(d, false);
+    const int64_t n = norm_bwd_groups(rows, norm_plan<T>(d, true)), m = norm_bwd_groups(rows, plan);
+    return ((size_t)(n > m ? n : m) * 2 * (size_t)d + (size_t)(plan.nv == 0 ? rows : 0)) * sizeof(typename NormAcc<T>::type);
 }
 
 template <typename T>
@@ -442,8 +486,9 @@ static int norm_bwd_impl(const void *x, int64_t rows, int64_t d, int64_t x_rs, c
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", ws_bytes, norm_bwd_bytes<T>(rows, d));
     const NormPlan plan = norm_plan<T>(d, norm_aligned<T>(d, x, x_rs, dy, dy_rs, dx, w, nullptr));
     const int64_t groups = norm_bwd_groups(rows, plan);
-    NormArgs<T> a{(const T *)x, (const T *)dy, (T *)dx, w, nullptr, (A *)mean, (A *)rstd, sums ? (A *)ws : nullptr, rows, d, x_rs, dy_rs,
-                  wide, 0.0};
+    NormArgs<T> a{(const T *)x, (const T *)dy, (T *)dx, w, nullptr, (A *)mean, (A *)rstd, sums ? (A *)ws : nullptr, nullptr, rows, d,
+                  x_rs, dy_rs, wide, 0.0};
+    if (sums && plan.nv == 0) a.shift = a.partial + groups * 2 * d;
     if (plan.vec == 1) norm_backward<T, 1>(a, plan, groups, st);
     else norm_backward<T, 16 / sizeof(T)>(a, plan, groups, st);
     FLK_LAUNCH_CHECK("layer_norm_bwd_kernel");
