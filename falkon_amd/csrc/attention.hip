@@ -111,13 +111,14 @@ static int parts_for(int64_t groups, int64_t keys, int dtype) {
     return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }
 
-struct AttnSizes { int64_t doc_blocks, docs, sq_pad, stats, bad, slopes, dq, dkv; int parts, head_parts, row_parts; };
+struct AttnSizes { int64_t doc_blocks, docs, sq_pad, stats, sizes, bad, slopes, dq, dkv; int parts, head_parts, row_parts; };
 static AttnSizes attn_sizes(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hk, int64_t d, int64_t dv, bool docs, bool slopes, int dtype) {
     AttnSizes z = {};
     z.doc_blocks = cdiv(sk, kDocBlock);
     z.docs = docs ? doc_bytes(b, sk) : 0;
     z.sq_pad = cdiv(sq, kAttnRows) * kAttnRows;
     z.stats = align256((size_t)(b * hq * z.sq_pad) * 12);
+    z.sizes = dtype == FLK_F16 ? align256((size_t)(b * hq * z.sq_pad / 32) * 8) : 0;
     z.bad = align256((size_t)(b * hq * z.sq_pad / 32));
     z.slopes = slopes ? align256((size_t)(b * hq * cdiv(sq, kAttnRows)) * 4) : 0;
     // (the slopes' gradient is a product of two of a row's sums, so their rows are not divided)
@@ -298,7 +299,7 @@ size_t flk_attention_backward_workspace_bytes(int64_t b, int64_t sq, int64_t sk,
     if (b < 0 || sq < 0 || sk < 0 || hq < 1 || hk < 1 || d < 1 || dv < 1 || hq % hk != 0 || sq > kMaxPositions || sk > kMaxPositions || !attn_dtype(dtype))
         return 0;
     const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, with_documents != 0, with_slopes != 0, dtype);
-    return (size_t)(z.docs + z.stats + z.bad + z.slopes + z.dq + z.dkv);
+    return (size_t)(z.docs + z.stats + z.sizes + z.bad + z.slopes + z.dq + z.dkv);
 }
 
 int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h, const void *k, int64_t k_b, int64_t k_s, int64_t k_h,
@@ -315,7 +316,7 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     if ((b * sq > 0 && (q == nullptr || out == nullptr || lse == nullptr || dout == nullptr)) || (b * sk > 0 && (k == nullptr || v == nullptr)))
         return fail(FLK_EINVAL, "flk_attention_backward: null pointer");
     const AttnSizes z = attn_sizes(b, sq, sk, hq, hk, d, dv, documents != nullptr, dslopes != nullptr, dtype);
-    const size_t need = (size_t)(z.docs + z.stats + z.bad + z.slopes + z.dq + z.dkv);
+    const size_t need = (size_t)(z.docs + z.stats + z.sizes + z.bad + z.slopes + z.dq + z.dkv);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(FLK_ENOMEM, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     AttnArgs a = {};
@@ -329,6 +330,7 @@ int flk_attention_backward(const void *q, int64_t q_b, int64_t q_s, int64_t q_h,
     char *ws = (char *)workspace;
     place_docs(a, ws); ws += z.docs;
     a.stats = (float *)ws; ws += z.stats;
+    a.sizes = (float2 *)ws; ws += z.sizes;
     a.bad_rows = (unsigned char *)ws; ws += z.bad;
     a.dslopes_part = dslopes != nullptr ? (float *)ws : nullptr; ws += z.slopes;
     a.dq_part = (float *)ws; ws += z.dq;

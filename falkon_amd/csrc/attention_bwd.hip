@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     const T *grow = (const T *)p.dout + b * p.dos.b + h * p.dos.h + (int64_t)row * p.dos.s;
     const int64_t at = (((int64_t)b * p.sq + row) * p.hq + h) * p.dv_d;
     frag qf[C], gf[C];
-    float delta = 0.f;
+    float delta = 0.f, size = 0.f;                                 // size: squared norm of dout
     unsigned bits = 0;
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -65,7 +65,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         gf[c] = g.f;
         bits |= bad_bits<T>(x.u) | bad_bits<T>(g.u);
 #pragma unroll
-        for (int i = 0; i < AT::E; i++) delta += (float)g.f[i] * ((float)o.f[i] + (float)e.f[i]);
+        for (int i = 0; i < AT::E; i++) {
+            delta += (float)g.f[i] * ((float)o.f[i] + (float)e.f[i]);
+            if constexpr (kNarrow<T>) size += (float)g.f[i] * (float)g.f[i];
+        }
     }
     delta += other_half(delta);
     // the statistics of this tile's rows, for both kernels; a row that sees nothing, or is none, has every p zero
@@ -81,6 +84,13 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         st[0] = bad_row ? kInf : lse;
         st[p.sq_pad] = delta;
         st[2 * p.sq_pad] = lse;
+    }
+    if constexpr (kNarrow<T>) {                                    // of rows that are finite and see something
+        size += other_half(size);
+        const bool counts = lse != kInf && !bad_row && __builtin_fabsf(delta) < kInf;
+        float2 top = {__builtin_sqrtf(wave_maxf(counts ? size : 0.f)), wave_maxf(counts ? __builtin_fabsf(delta) : 0.f)};
+        if (__any(bad_row)) top.x = -top.x;                        // (so that the other kernel has one thing to ask for; -0 too)
+        if (lane == 0 && part == 0) p.sizes[(((int64_t)b * p.hq + h) * p.sq_pad + i0) / 32 + wave] = top;
     }
     const int bad_wave = (__any(bad_row) ? 1 : 0) | (__any(bad_row && lse != kInf) ? 2 : 0);
     if (lane == 0 && part == 0) p.bad_rows[(((int64_t)b * p.hq + h) * p.sq_pad + i0) / 32 + wave] = (unsigned char)bad_wave;
@@ -121,6 +131,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     fx16 acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) acc[db] = fx16{};
+    // float16: the scores' gradients of a row (and its sums) are held times 2^lift.  The shift is a part of lse; it begins so high that
+    // nothing is lost and falls where a tile would exceed 2^15 (as a running maximum does; then to 2^7, so that it seldom falls again).
+    constexpr float kFirstLift = kNarrow<T> ? 40.f : 0.f;
+    float lift = kFirstLift, lse_lift = lse - kFirstLift;
     // sum_j dS |dist|, sum_j dS and sum_j P |dist|: the second is what the rounding of out left in delta, and is taken out
     float far = 0.f, left = 0.f, reach = 0.f;
 
@@ -169,8 +183,8 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
             for (int r = 0; r < 16; r++) {
                 float e, g, grad = 1.f;
                 const float dist = at_key - (float)(32 * kb + 8 * (r >> 2) + (r & 3));
-                if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse));
-                else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse);
+                if constexpr (MOD == kPlain) e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], score.unit, -lse_lift));
+                else e = __builtin_amdgcn_exp2f(score(s[r], dist, grad) - lse_lift);
                 g = e * (dp[r] - delta);
                 if (!full) g = seen.or_zero(g, kb, r);
                 if constexpr ((MOD & kDecay) != 0 && !decltype(careful)::value) {
@@ -183,6 +197,23 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                 }
                 if constexpr ((MOD & kCap) != 0) g *= grad;
                 s[r] = g;
+            }
+            if constexpr (kNarrow<T>) {
+                float top = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) top = fmaxf(top, __builtin_fabsf(s[r]));
+                if (__any(top > 32768.f)) {
+                    top = fmaxf(top, other_half(top));
+                    const float drop = top > 32768.f ? (float)(__builtin_amdgcn_frexp_expf(fminf(top, 1e38f)) - 7) : 0.f;
+                    const float by = __builtin_amdgcn_exp2f(-drop);
+                    lift -= drop;
+                    lse_lift += drop;
+                    if constexpr (!decltype(careful)::value) { far *= by; left *= by; reach *= by; }
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[r] *= by;
+#pragma unroll
+                    for (int db = 0; db < DB; db++) acc[db] *= by;
+                }
             }
             FLK_KEEP_ORDER();
 #pragma unroll
@@ -231,10 +262,13 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     // product with the keys, and are masked.)
     if (bad) lds_bad = 1;
     __syncthreads();
+    const float unlift = __builtin_amdgcn_exp2f(-lift);            // of the slopes' sums
     const bool again = p.dq != nullptr && lds_bad != 0;
     if (again) {
 #pragma unroll
         for (int db = 0; db < DB; db++) acc[db] = fx16{};
+        lift = kFirstLift;
+        lse_lift = lse - kFirstLift;
         lds_spoilt[wave * 32 + (lane & 31)].clear();
         walk.start((int)(tiles_k * part / p.parts), (int)(tiles_k * (part + 1) / p.parts));
         while ((tile = walk.next(look)) >= 0) {
@@ -255,7 +289,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
         far += other_half(far);
         left += other_half(left);
         reach += other_half(reach);
-        float x = live && half == 0 ? left * reach - far : 0.f;
+        float x = live && half == 0 ? (left * (reach * unlift) - far) * unlift : 0.f;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
         if (lane == 0) lds_sum[wave] = x;
@@ -266,7 +300,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     if (p.dq == nullptr) return;
     __syncthreads();
     if (again) lds_spoilt[wave * 32 + (lane & 31)].mark(acc);
-    const float unscale = p.scale * score.kGrad;
+    const float unscale = p.scale * score.kGrad * __builtin_amdgcn_exp2f(-lift);
     const int64_t to = (((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h) * p.d, row_q = (int64_t)p.hq * p.d;
     const auto value = [&](int db, int r) { return acc[db][r] * unscale; };
     const int rows = p.sq - (i0 + wave * 32);
@@ -290,6 +324,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     __shared__ __align__(16) float lds_stat[2][2][TQ];             // lse and delta of a tile's rows
     __shared__ int lds_doc[8];
     __shared__ int lds_bad[4];
+    __shared__ float lds_size[4][3];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int pairs = p.b * p.hk, tiles_k = (p.sk + kAttnRows - 1) / kAttnRows;
@@ -313,13 +348,22 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int head_end = p.group * (head_part + 1) / p.head_parts;
     // Whether any of the rows that this workgroup goes over is not finite.  (Asked for first, so that the answer is on its way together
     // with keys and values.)
+    // float16: also the largest norm of a row of dout, and |delta|.
     bool bad = false;
-    {
-        const int n = (walk_end * TQ + kAttnRows - 1) / kAttnRows - walk_lo * TQ / kAttnRows, all = n * (head_end - head);
+    float dout_size = 0.f, delta_size = 0.f;
+    const int64_t line0 = (int64_t)b * p.hq + hk * p.group + head;
+    if constexpr (kNarrow<T>) {
+        const int first_of = walk_lo * TQ / 32, n = walk_end * TQ / 32 - first_of, all = n * (head_end - head);
         for (int i = threadIdx.x; i < all; i += kAttnThreads) {
-            const int64_t of = (int64_t)b * p.hq + hk * p.group + head + i / n;
-            bad |= ((const int *)p.bad_rows)[of * (p.sq_pad / kAttnRows) + walk_lo * TQ / kAttnRows + i % n] != 0;
+            const float2 x = p.sizes[(line0 + i / n) * (p.sq_pad / 32) + first_of + i % n];
+            bad |= __builtin_signbitf(x.x);
+            dout_size = fmaxf(dout_size, __builtin_fabsf(x.x));
+            delta_size = fmaxf(delta_size, x.y);
         }
+    } else {
+        const int first_of = walk_lo * TQ / kAttnRows, n = (walk_end * TQ + kAttnRows - 1) / kAttnRows - first_of, all = n * (head_end - head);
+        for (int i = threadIdx.x; i < all; i += kAttnThreads)
+            bad |= ((const int *)p.bad_rows)[(line0 + i / n) * (p.sq_pad / kAttnRows) + first_of + i % n] != 0;
     }
     const T *krow = (const T *)p.k + b * p.ks.b + hk * p.ks.h + (int64_t)key * p.ks.s;
     const T *vrow = (const T *)p.v + b * p.vs.b + hk * p.vs.h + (int64_t)key * p.vs.s;
@@ -340,6 +384,23 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
     const bool bad_wave = __any(bad);
     if (lane == 0) lds_bad[wave] = bad_wave;
+    // float16: weights are held times 2^14, and the scores' gradients times 2^14 and a power of two, `fit`, that bounds them by 2^15:
+    // |dP - delta| is at most the largest norm of a row of dout times that of a key's row of v, plus the largest |delta|.
+    constexpr float kLift = kNarrow<T> ? 14.f : 0.f;
+    float fit = 1.f;
+    if constexpr (kNarrow<T>) {
+        float v_size = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < AT::E; i++) v_size += (float)vf[c][i] * (float)vf[c][i];
+        v_size += other_half(v_size);
+        v_size = v_size < kInf ? v_size : 0.f;
+        dout_size = wave_maxf(dout_size);
+        delta_size = wave_maxf(delta_size);
+        v_size = wave_maxf(v_size);
+        if (lane == 0) { lds_size[wave][0] = dout_size; lds_size[wave][1] = delta_size; lds_size[wave][2] = v_size; }
+    }
     if (p.docs != nullptr) {
         const int raw = live ? ids[key] : -1;
         span = {wave_min(raw), wave_max(raw)};
@@ -348,6 +409,13 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     }
     __syncthreads();
     bad = (lds_bad[0] | lds_bad[1] | lds_bad[2] | lds_bad[3]) != 0;
+    if constexpr (kNarrow<T>) {
+        float x[3];
+#pragma unroll
+        for (int i = 0; i < 3; i++) x[i] = fmaxf(fmaxf(lds_size[0][i], lds_size[1][i]), fmaxf(lds_size[2][i], lds_size[3][i]));
+        const float most = 1.01f * (x[0] * __builtin_sqrtf(x[2]) + x[1]);
+        if (most > 0.f) fit = __builtin_amdgcn_exp2f((float)(1 - max(__builtin_amdgcn_frexp_expf(most), -100)));
+    }
     if (p.docs != nullptr) {
         wg_span.x = min(min(lds_doc[0], lds_doc[1]), min(lds_doc[2], lds_doc[3]));
         wg_span.y = max(max(lds_doc[4], lds_doc[5]), max(lds_doc[6], lds_doc[7]));
@@ -391,7 +459,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
         if (p.docs != nullptr) next_id = lane < rows ? ids[i0 + off + lane] : -1;
     };
     const auto put = [&](int to) {
-        if (mine) { lds_stat[to][0][threadIdx.x] = r_lse; lds_stat[to][1][threadIdx.x] = r_delta; }
+        if (mine) { lds_stat[to][0][threadIdx.x] = r_lse - kLift; lds_stat[to][1][threadIdx.x] = r_delta * fit; }
     };
     TileWalk walk, again;
     walk.start(walk_lo, walk_end);
@@ -481,7 +549,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
                         float grad = 1.f;
                         if constexpr (MOD == kPlain) e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][r], score.unit, -li));
                         else e[k] = __builtin_amdgcn_exp2f(score(s[qb][r], at_row + (float)(32 * qb + 8 * (r >> 2) + (r & 3)), grad) - li);
-                        float x = dp[qb][r] - de;
+                        float x = kNarrow<T> ? __builtin_fmaf(dp[qb][r], fit, -de) : dp[qb][r] - de;
                         if constexpr ((MOD & kCap) != 0) x *= grad;
                         if (masked) e[k] = seen.or_zero(e[k], qb, r);
                         g[k] = times_or_zero(e[k], x);                       // a hidden place stays zero whatever x is
@@ -563,19 +631,19 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
         }
     }
     __syncthreads();
-    const float unscale = p.scale * Score<T, MOD>::kGrad;
+    const float lowered = __builtin_amdgcn_exp2f(-kLift), unscale = p.scale * Score<T, MOD>::kGrad * lowered / fit;
     const int rows = p.sk - k_lo;
     const int64_t line = (int64_t)b * p.sk + k_lo, at_k = (line * p.hk + hk) * p.d, at_v = (line * p.hk + hk) * p.dv_d;
     const int64_t row_k = (int64_t)p.hk * p.d, row_v = (int64_t)p.hk * p.dv_d;
     if (splits == 1) {
         char *mine = lds + wave * 32 * TL::RB;
         store_rows<T, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, (T *)p.dk + at_k, row_k, rows, p.d, p.vec);
-        store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r]; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec_v);
+        store_rows<T, DP>(mine, [&](int db, int r) { return dv[db][r] * lowered; }, (T *)p.dv + at_v, row_v, rows, p.dv_d, p.vec_v);
     } else {                                                       // parts in float, added by attention_join_kernel
         const int64_t nk = (int64_t)p.b * p.sk * row_k, nv = (int64_t)p.b * p.sk * row_v;
         char *mine = lds + wave * 32 * Tile<float, DP>::RB;
         store_rows<float, DP>(mine, [&](int db, int r) { return dk[db][r] * unscale; }, p.dkv_part + split * nk + at_k, row_k, rows, p.d, p.d % 4 == 0);
-        store_rows<float, DP>(mine, [&](int db, int r) { return dv[db][r]; }, p.dkv_part + splits * nk + split * nv + at_v, row_v, rows, p.dv_d,
+        store_rows<float, DP>(mine, [&](int db, int r) { return dv[db][r] * lowered; }, p.dkv_part + splits * nk + split * nv + at_v, row_v, rows, p.dv_d,
                               p.d % 4 == 0 && p.dv_d % 4 == 0);
     }
 }

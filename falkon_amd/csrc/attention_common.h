@@ -127,6 +127,10 @@ template <typename T, int DP> struct Tile {
     }
 };
 
+// Weights of float16 data are held times 2^kLift (or more) where they are rounded: its normal numbers end at 6e-5, which a row of 16 000
+// keys reaches, and rounding below that costs digits (below 3e-8, everything).  The shift is part of the exponent and costs nothing.
+template <typename T> constexpr bool kNarrow = std::is_same<T, f16_t>::value;
+
 // KS accumulator registers from r0 on as the second operand of a product over their rows.  The rounding of p (and of its
 // gradient) to 16 bits is what feeds the matrix cores at their full rate; p lies in [0, 1] before the final division, its
 // rounding errors are independent, and the sums of p itself are of the unrounded values.
@@ -160,6 +164,7 @@ struct AttnArgs {
     // backward: [b][hq][3][sq_pad], the rows' lse (in units of log 2; infinite, so that weights are zero, for a row of q or dout that holds
     // infinities or NaNs), delta, and the lse without that
     float *stats;
+    float2 *sizes;                                     // backward of float16: [b][hq][sq_pad / 32], largest norm of 32 rows of dout (negative: bad_rows) and |delta|
     unsigned char *bad_rows;                           // backward: [b][hq][sq_pad / 32], whether there is such a row among 32 (1) that sees something (2)
     int64_t sq_pad;
     AttnStride qs, ks, vs, dos;                        // strides of q, k, v and dout; the others are contiguous
@@ -473,6 +478,12 @@ __device__ __forceinline__ int wave_max(int x) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
     return __builtin_amdgcn_readfirstlane(x);
+}
+
+__device__ __forceinline__ float wave_maxf(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
 }
 
 // smallest and largest document id of positions [lo, hi), a padding position counting as -1; (0, -1) if there is none
