@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(64 * W, W > 4 || (sizeof(T) == 4 && DP > 64) ?
 #pragma unroll
             for (int db = 0; db < DB; db++) o[db] *= a;
         }
-        const float base_m = m == -kInf ? 0.f : m;
+        constexpr float kLift = kNarrow<T> ? 14.f : 0.f;           // (the same for all parts: their maxima join them as they are)
+        const float base_m = m == -kInf ? 0.f : m - kLift;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(s[i] - base_m);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};                       // short chains: long ones would cost float data digits

@@ -127,8 +127,8 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// Weights of float16 data are held times 2^kLift (or more) where they are rounded: its normal numbers end at 6e-5, which a row of 16 000
-// keys reaches, and rounding below that costs digits (below 3e-8, everything).  The shift is part of the exponent and costs nothing.
+// Weights of float16 data are held times 2^8 or more where they are rounded: its normal numbers end at 6e-5, which the weights of a row of
+// 16 000 keys reach, and rounding below that costs digits (below 3e-8, everything).  The shift is part of the exponent and costs nothing.
 template <typename T> constexpr bool kNarrow = std::is_same<T, f16_t>::value;
 
 // KS accumulator registers from r0 on as the second operand of a product over their rows.  The rounding of p (and of its

@@ -10,6 +10,8 @@ namespace flk {
 // A maximum is taken over only when a row exceeds the present one by this much (in units of log 2): weights then lie below
 // 2^kSlack, which every type holds, and most tiles after the first need no rescaling.
 constexpr float kSlack = 6.f;
+// ... and float16's lie between 2^14 for the largest and 2^-14, the last normal number, for one of 2^-22 of the maximum
+template <typename T> constexpr float kLift = kNarrow<T> ? 8.f : 0.f;
 
 template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) attention_fwd_kernel(AttnArgs p) {
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
 #pragma unroll
                 for (int db = 0; db < DB; db++) o[db] *= a;
             }
-            const float base_m = m == -kInf ? 0.f : m;
+            const float base_m = m == -kInf ? 0.f : m - kLift<T>;
             // Weights and their product with the values.  The first fragments of the values are on their way before the first
             // weights are formed; the weights of the next 32 keys are formed between the products of the present ones.
             float sum[4] = {0.f, 0.f, 0.f, 0.f};                   // short chains: long ones would cost float data digits
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
                               p.part_o + (part * rows_all + first) * p.dv_d, (int64_t)p.hq * p.dv_d, p.sq - (i0 + wave * 32), p.dv_d, p.dv_d % 4 == 0);
         if (live && half == 0) {
             float *ml = p.part_ml + (part * rows_all + first + (int64_t)lane * p.hq) * 2;
-            ml[0] = m;
+            ml[0] = m - kLift<T>;
             ml[1] = l;
         }
         return;
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r] - (float)(T)o[db][r]; }, (T *)p.rest + at, row_o, rows, p.dv_d, p.vec_v);
     if (!live) return;
     if (half == 0 && p.lse != nullptr)
-        p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : m * kLn2 + __logf(l);
+        p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : (m - kLift<T>) * kLn2 + __logf(l);
 }
 
 template <typename T> int launch_attention_fwd(const AttnArgs &a, int dp, hipStream_t st) {

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from falkon_amd import attention
+from falkon_amd import attention, cached_attention
 
 from attention_ref import reference
 
@@ -72,3 +72,21 @@ def test_rows_of_dout_of_very_different_sizes():
     for name, t in zip(("dq", "dk", "dv"), big):
         assert bool(t.isfinite().all())
         assert float((t - exact[name][0]).norm()) <= 2.0 ** -9 * float(exact[name][0].norm()), name
+
+
+@pytest.mark.gpu
+def test_a_peak_over_a_long_tail():
+    """One key's weight is twice those of 130 000 others together: 2^-18 of it each.  The parts of a row's keys join exactly, so there are
+    enough rows that their keys are not divided."""
+    n, d, heads = 130_001, 32, 512
+    q = torch.zeros(1, 1, heads, d, device=DEV, dtype=torch.float16)
+    k = torch.zeros(1, n, 1, d, device=DEV, dtype=torch.float16)
+    v = (1 + torch.rand(1, n, 1, d, generator=torch.Generator().manual_seed(53))).half().to(DEV)
+    q[..., 0], k[:, 77, :, 0] = 3.5, 3.5625                                  # exp(12.47) = 2.6e5
+    v[:, 77] = 0
+    want = reference(q[:, :, :1], k, v, scale=1.0)["out"][0]
+    # half a step, 2^-11, for the result, for the peak's weight and for the tail's, which are rounded alike, all being equal
+    got = attention(q, k, v, scale=1.0)
+    assert bool(((got.double().cpu() - want).abs() <= 3 * 2.0 ** -11 * want.abs()).all())
+    got = cached_attention(q[:, 0, :1], k, v, torch.tensor([n], device=DEV), scale=1.0)
+    assert bool(((got.double().cpu() - want[:, 0]).abs() <= 3 * 2.0 ** -11 * want[:, 0].abs()).all())
