@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     }
     const int bad_wave = (__any(bad_row) ? 1 : 0) | (__any(bad_row && lse != kInf) ? 2 : 0);
     if (lane == 0 && part == 0) p.bad_rows[(((int64_t)b * p.hq + h) * p.sq_pad + i0) / 32 + wave] = (unsigned char)bad_wave;
+    if (p.dq == nullptr && p.dslopes_part == nullptr) return;      // only dk and dv are wanted
 
     int id = 0;
     int2 span = {0, 0}, wg_span = {0, 0};
