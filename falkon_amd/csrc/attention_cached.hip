@@ -119,6 +119,9 @@ __global__ void __launch_bounds__(64 * W, W > 4 || (sizeof(T) == 4 && DP > 64) ?
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
         for (int st = 0; st < ST; st++) {
+            // 16-bit weights are rounded once, as in the other kernels.  (In two pieces, the second holding what rounding took from the first,
+            // results are those of 32 bits, 1.67e-3 from the exact ones where these are 1.81e-3, almost all of it their own rounding;
+            // 64 sequences of up to 16 384 keys take 510 us so instead of 434.)
             const frag pf = pack<T>(s, st);
 #pragma unroll
             for (int db = 0; db < DB; db++) {
