@@ -385,9 +385,10 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
     const int *ids = p.doc_ids + (int64_t)b * p.doc_blocks * kDocBlock;
     const bool bad_wave = __any(bad);
     if (lane == 0) lds_bad[wave] = bad_wave;
-    // float16: weights are held times 2^14, and the scores' gradients times 2^14 and a power of two, `fit`, that bounds them by 2^15:
-    // |dP - delta| is at most the largest norm of a row of dout times that of a key's row of v, plus the largest |delta|.
-    constexpr float kLift = kNarrow<T> ? 14.f : 0.f;
+    // float16: weights are held times 2^10, and the scores' gradients times 2^10 and a power of two, `fit`, that bounds them by 2^11:
+    // |dP - delta| is at most the largest norm of a row of dout times that of a key's row of v, plus the largest |delta|.  (Five more
+    // bits are left, since a weight exceeds one by the rounding of scores of millions.)
+    constexpr float kLift = kNarrow<T> ? 10.f : 0.f;
     float fit = 1.f;
     if constexpr (kNarrow<T>) {
         float v_size = 0.f;

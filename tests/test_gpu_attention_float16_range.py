@@ -90,3 +90,12 @@ def test_a_peak_over_a_long_tail():
     assert bool(((got.double().cpu() - want).abs() <= 3 * 2.0 ** -11 * want.abs()).all())
     got = cached_attention(q[:, 0, :1], k, v, torch.tensor([n], device=DEV), scale=1.0)
     assert bool(((got.double().cpu() - want[:, 0]).abs() <= 3 * 2.0 ** -11 * want[:, 0].abs()).all())
+
+
+@pytest.mark.gpu
+def test_gradients_of_scores_of_millions():
+    """float's step at 1e7 is one, so a weight may come out as e^(1/2): nothing overflows behind it."""
+    q, k, v, do = _make(1, 200, 200, 2, 2, 64, 54)
+    q, k = q * 900, k * 900
+    for t in _grads(q, k, v, do.half(), causal=True):
+        assert bool(t.isfinite().all())
