@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     __shared__ __align__(16) char lds[4 * kTileBytes];
     __shared__ int lds_doc[8];
     __shared__ float lds_sum[4];
+    __shared__ float lds_lse[kNarrow<T> ? kAttnThreads : 1];
     __shared__ int lds_bad;
     __shared__ Spoilt<DP> lds_spoilt[kAttnRows];
 
@@ -134,8 +135,10 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
     for (int db = 0; db < DB; db++) acc[db] = fx16{};
     // float16: the scores' gradients of a row (and its sums) are held times 2^lift.  The shift is a part of lse; it begins so high that
     // nothing is lost and falls where a tile would exceed 2^15 (as a running maximum does; then to 2^7, so that it seldom falls again).
+    // (What remains of lse is small then and has all its digits: the slopes' gradient, in float, would show less.)
     constexpr float kFirstLift = kNarrow<T> ? 40.f : 0.f;
     float lift = kFirstLift, lse_lift = lse - kFirstLift;
+    if constexpr (kNarrow<T>) lds_lse[threadIdx.x] = lse;
     // sum_j dS |dist|, sum_j dS and sum_j P |dist|: the second is what the rounding of out left in delta, and is taken out
     float far = 0.f, left = 0.f, reach = 0.f;
 
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
                     const float drop = top > 32768.f ? (float)(__builtin_amdgcn_frexp_expf(fminf(top, 1e38f)) - 7) : 0.f;
                     const float by = __builtin_amdgcn_exp2f(-drop);
                     lift -= drop;
-                    lse_lift += drop;
+                    lse_lift = lds_lse[threadIdx.x] - lift;
                     if constexpr (!decltype(careful)::value) { far *= by; left *= by; reach *= by; }
 #pragma unroll
                     for (int r = 0; r < 16; r++) s[r] *= by;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kAttnThreads, sizeof(T) == 4 && DP > 64 ? 1 : 
 #pragma unroll
         for (int db = 0; db < DB; db++) acc[db] = fx16{};
         lift = kFirstLift;
-        lse_lift = lse - kFirstLift;
+        if constexpr (kNarrow<T>) lse_lift = lds_lse[threadIdx.x] - lift;
         lds_spoilt[wave * 32 + (lane & 31)].clear();
         walk.start((int)(tiles_k * part / p.parts), (int)(tiles_k * (part + 1) / p.parts));
         while ((tile = walk.next(look)) >= 0) {

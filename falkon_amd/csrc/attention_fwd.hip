@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         skip = walk.is_skip;
     }
     l += other_half(l);
+    constexpr float kUnlift = 1.f / (1 << (int)kLift<T>);          // (exact, and the logarithm is as exact as without)
     if (few) {
 #pragma unroll
         for (int c = 0; c < 4; c++) o[0][c] += other_half(o[0][c]);
@@ -257,12 +258,12 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
     if (p.parts > 1) {                                             // joined by attention_parts_kernel
         const int64_t rows_all = (int64_t)p.b * p.sq * p.hq, first = ((int64_t)b * p.sq + i0 + wave * 32) * p.hq + h;
         __syncthreads();
-        store_rows<float, DP>(lds + wave * 32 * Tile<float, DP>::RB, [&](int db, int r) { return o[db][r]; },
+        store_rows<float, DP>(lds + wave * 32 * Tile<float, DP>::RB, [&](int db, int r) { return o[db][r] * kUnlift; },
                               p.part_o + (part * rows_all + first) * p.dv_d, (int64_t)p.hq * p.dv_d, p.sq - (i0 + wave * 32), p.dv_d, p.dv_d % 4 == 0);
         if (live && half == 0) {
             float *ml = p.part_ml + (part * rows_all + first + (int64_t)lane * p.hq) * 2;
-            ml[0] = m - kLift<T>;
-            ml[1] = l;
+            ml[0] = m;
+            ml[1] = l * kUnlift;
         }
         return;
     }
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
         store_rows<T, DP>(mine, [&](int db, int r) { return o[db][r] - (float)(T)o[db][r]; }, (T *)p.rest + at, row_o, rows, p.dv_d, p.vec_v);
     if (!live) return;
     if (half == 0 && p.lse != nullptr)
-        p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : (m - kLift<T>) * kLn2 + __logf(l);
+        p.lse[((int64_t)b * p.hq + h) * p.sq + row] = l == 0.f ? -kInf : m * kLn2 + __logf(l * kUnlift);
 }
 
 template <typename T> int launch_attention_fwd(const AttnArgs &a, int dp, hipStream_t st) {
