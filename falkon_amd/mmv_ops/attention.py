@@ -9,11 +9,12 @@ row divided by its sum, as a kernel smoother (Nadaraya-Watson) or an attention l
     out_i = sum_j softmax_j(x_ij) v_j                          over the keys j that row i sees
 
 The queries stand at the newest positions of the keys: ``pos_i = i + (number of keys) - (number of queries)``.  A row that
-sees no key is zero.  Keys that no row sees leave no trace in a result or a gradient, whatever they hold (NaN included);
-neither does a NaN or an infinity of a key reach a row that does not see it.
+sees no key, or none with a score above minus infinity, is zero.  Keys that no row sees leave no trace in a result or a gradient, whatever
+they hold (NaN included); neither does a NaN or an infinity of a key reach a row that does not see it, nor one of a row the keys that it
+does not see.  What sees them gets what the formula gives in 32 bits (zero times an infinity is NaN).
 
 Scores, maxima, sums and outputs are held in 32 bits; for 16-bit data the weights (and their gradients) are rounded to
-that type before the second product, which is what the matrix cores take.  Scores of more than 1e9 in size are beyond statistics
+that type before the second product, which is what the matrix cores take (float16's shifted, so that small ones keep their digits).  Scores of more than 1e9 in size are beyond statistics
 in 32 bits (a rounding of one is more than an exponent holds): such a row may be NaN.  Results and gradients are the same run to run.
 The reference has no counterpart.  The work is done by ``flk_attention``, ``flk_attention_backward`` and
 ``flk_attention_cached``; nothing is computed on the CPU.

@@ -94,7 +94,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         ``x``, float32.
     eps : added to the variance.
 
-    Returns a new contiguous tensor like ``x``.  Sums are held in 32 bits (64 for float64) and results rounded once.
+    Returns a new contiguous tensor like ``x``.  Sums are held in 32 bits (64 for float64) and results rounded once; rows far from zero
+    are as exact as others (a constant row is zero).
     Differentiable in ``x``, ``weight`` and ``bias`` (once); gradients are the same run to run.  The call is
     asynchronous on the current stream and can be captured into a graph; to capture its backward pass, first let go of every
     eager result that was computed from the same leaves (torch ties a leaf's gradient to the stream of the first graph alive,
