@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kAttnThreads, (kAlone<T, DP> ? 1 : 2)) attenti
 // What rows of q and dout with infinities or NaNs, which have no weight in the kernel above, do to dk and dv of the keys that see
 // them: one row after the other, by vector instructions, added to what was written (to the first of its parts).  A product of matrices
 // would carry their NaNs (zero times an infinity) to the keys that do not see them.  A workgroup goes over the rows for 128 keys, and has
-// nothing to do where all rows are finite (3 us; as a branch of the kernel above it took 5 % of its time by its registers).
+// nothing to do where all rows are finite (4 to 5 us; as a branch of the kernel above it took 5 % of its time by its registers).
 template <typename T, int DP, int MOD>
 __global__ void __launch_bounds__(kAttnThreads) attention_bad_rows_kernel(AttnArgs p) {
     typedef AttnType<T> AT;

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kAttnThreads, (sizeof(T) == 2 && DP <= 64 ? 3 
 
     // Up to four float outputs a row, as a regression has them, would leave most of a matrix instruction's 32 columns empty, each
     // of them as dear as a column of the scores' product: their sums are made by vector instructions, each half of the
-    // lanes for its keys, in the first four registers of o (1e5 rows of 28 features, 2000 keys, 4 outputs: 326 -> 257 us).
+    // lanes for its keys, in the first four registers of o (1e5 rows of 28 features, 2000 keys, 4 outputs: 326 us without this, 267 with it).
     const bool few = sizeof(T) == 4 && DP <= 64 && p.dv_d <= 4;     // (wider heads have no registers to spare)
     fx16 o[DB];
 #pragma unroll

@@ -241,3 +241,68 @@ def test_gradients_where_nothing_is_finite(dtype):
     want = _grads(q, k, v, do, causal=True, documents=ids)
     q[:, 200:600], do[:, 250:600] = float("nan"), float("inf")
     assert all(torch.equal(a, b) for a, b in zip(_grads(q, k, v, do, causal=True, documents=ids), want))
+
+
+def _by_the_formula(q, k, v, do, see, scale, cap, slopes):
+    """out, dq, dk and dv of one batch entry in 64 bits, place by place over what is seen, with IEEE's rules for what is not finite."""
+    g = q.shape[1] // k.shape[1]
+    q, k, v, do = (t.double().cpu().transpose(0, 1) for t in (q, k, v, do))
+    sq, sk = q.shape[1], k.shape[1]
+    dist = (torch.arange(sk - sq, sk)[:, None] - torch.arange(sk)[None]).abs().double()
+    out, dq, dk, dv = torch.zeros_like(do), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    seen = lambda t: torch.where(see[:, :, None], t, 0.0)  # noqa: E731
+    for h in range(q.shape[0]):
+        kh, vh = k[h // g], v[h // g]
+        x, grad = scale * (q[h][:, None] * kh[None]).sum(2), 1.0
+        if cap:
+            t = torch.tanh(x / cap)
+            x, grad = cap * t, 1 - t * t
+        if slopes is not None:
+            x = x - float(slopes[h]) * dist
+        x = x.masked_fill(~see, -float("inf"))
+        lse = torch.logsumexp(x, 1, keepdim=True)
+        lse = torch.where(x.isnan().any(1, keepdim=True) | (x == float("inf")).any(1, keepdim=True), float("nan"), lse)
+        p = torch.exp(x - torch.where(lse == -float("inf"), 0.0, lse))
+        out[h] = seen(p[:, :, None] * vh[None]).sum(1)
+        dp, delta = (do[h][:, None] * vh[None]).sum(2), (do[h] * out[h]).sum(1, keepdim=True)
+        ds = p * (dp - delta) * grad
+        dq[h] = scale * seen(ds[:, :, None] * kh[None]).sum(1)
+        dk[h // g] += scale * seen(torch.where(p == 0, 0.0, ds)[:, :, None] * q[h][:, None]).sum(0)
+        dv[h // g] += seen(p[:, :, None] * do[h][:, None]).sum(0)
+    return [t.transpose(0, 1) for t in (out, dq, dk, dv)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("seed", range(12))
+def test_bad_values_scattered_over_all_operands(dtype, seed):
+    """A handful of infinities and NaNs anywhere: the same places are finite as by the formula, and those are as exact as ever.  (Where
+    a result is not finite, whether it is an infinity or NaN depends on how its sum is made.)"""
+    g = torch.Generator().manual_seed(100 + seed)
+    pick = lambda *a: a[int(torch.randint(len(a), (1,), generator=g))]  # noqa: E731
+    sq, sk, hq, hk, d, dv = pick(40, 130, 300), pick(45, 200, 1100), pick(2, 4), pick(1, 2), pick(16, 45, 80), pick(3, 32, 72)
+    q, k, v, do = _make(1, sq, sk, hq, hk, d, dv, dtype, seed=200 + seed)
+    q, k = q * 0.5, k * 0.7
+    causal, cap = pick(True, False), pick(0.0, 3.0)
+    slopes = pick(None, torch.linspace(0.0, 0.05, hq, device=DEV))
+    ids = pick(None, torch.arange(sk, device=DEV) * 3 // sk) if sq <= sk else None
+    prefix = pick(None, torch.tensor([20], device=DEV)) if causal else None
+    for t, many in ((q, pick(0, 2)), (k, pick(0, 2)), (v, pick(0, 2)), (do, pick(0, 2))):
+        for _ in range(many):
+            at = [int(torch.randint(n, (1,), generator=g)) for n in t.shape]
+            t[tuple(at)] = pick(float("inf"), -float("inf"), float("nan"))
+    pos, key = torch.arange(sk - sq, sk)[:, None], torch.arange(sk)[None]
+    see = key <= pos if causal else torch.ones(sq, sk, dtype=torch.bool)
+    if prefix is not None:
+        see = see | (key < 20)
+    if ids is not None:
+        see = see & (ids.cpu()[sk - sq:, None] == ids.cpu()[None])
+    want = _by_the_formula(q[0], k[0], v[0], do[0], see, 0.25, cap, slopes)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaves, scale=0.25, causal=causal, softcap=cap, slopes=slopes, prefix=prefix, documents=None if ids is None else ids[None].contiguous())
+    for name, got, value in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do)), want):
+        got, fine = got[0].double().cpu(), value.isfinite()
+        assert torch.equal(got.isfinite(), fine), name
+        if fine.any():                                                       # (weights, their gradients and the result: one rounding each)
+            unit = 2.0 ** -16 if dtype == torch.float32 else 2 * torch.finfo(dtype).eps
+            assert float((got - value)[fine].norm()) <= unit * float(value[fine].norm()) + 1e-6, name
