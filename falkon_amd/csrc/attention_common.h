@@ -127,8 +127,9 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// Weights of float16 data are held times 2^8 or more where they are rounded: its normal numbers end at 6e-5, which the weights of a row of
-// 16 000 keys reach, and rounding below that costs digits (below 3e-8, everything).  The shift is part of the exponent and costs nothing.
+// Whether the type's range is narrow: float16's normal numbers end at 6e-5, which the weights of a row of 16 000 keys reach, and rounding
+// below that costs digits (below 3e-8, everything).  Its weights are held times 2^8 or more where they are rounded; the shift is a part of
+// the exponent and costs nothing.
 template <typename T> constexpr bool kNarrow = std::is_same<T, f16_t>::value;
 
 // KS accumulator registers from r0 on as the second operand of a product over their rows.  The rounding of p (and of its
@@ -156,6 +157,7 @@ template <typename T> __device__ __forceinline__ void clean(char *at) {
     const ux4 u = *(const ux4 *)at;
     if (any_nonfinite<T>(u)) *(ux4 *)at = cleaned<T>(u);
 }
+
 struct AttnStride { int64_t b, s, h; };
 struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
